@@ -51,6 +51,7 @@ extern "C" {
 
 #define SVBGPU_ETOOBIG (-6)    /* count beyond SVBGPU_STATIC_MAX_COUNT
                                   (svbgpu_decode_static only)                    */
+#define SVBGPU_ENOMEM (-8)     /* host memory ran out (svbgpu_grad_clip only)    */
 
 const char *svbgpu_strerror(int code);
 
@@ -252,6 +253,59 @@ int svbgpu_quantize_encode(int variant, const float *d_in, uint32_t count, float
 int svbgpu_decode_dequantize(int variant, const uint8_t *d_in, float *d_out, uint32_t count,
                              float scale, int accumulate, void *d_workspace,
                              size_t workspace_bytes, uint64_t *d_consumed, void *stream);
+
+/*
+ * Gradient operators: what stands before and behind the two calls above in a training step.  No counterpart in the
+ * reference.
+ *
+ * A call takes a host array of tensors (any number, of mixed types, in any order, each aligned to its element type,
+ * empty ones allowed); it is read before the call returns and travels in kernel arguments, so a call can be captured
+ * into a graph and replayed.  Elements are counted as they lie in memory: a tensor is `count` consecutive elements.
+ * Workspace: svbgpu_grad_workspace_bytes(ntensors), 256-byte aligned, never initialised, for one call at a time.
+ */
+#define SVBGPU_F32 0
+#define SVBGPU_F16 1
+#define SVBGPU_BF16 2
+typedef struct svbgpu_tensor {
+  void *data;     /* device memory                         */
+  uint64_t count; /* elements, less than 2^37              */
+  int32_t type;   /* SVBGPU_F32, SVBGPU_F16 or SVBGPU_BF16 */
+} svbgpu_tensor;
+#define SVBGPU_NORM_MAX 0 /* max |x|        */
+#define SVBGPU_NORM_L1 1  /* sum |x|        */
+#define SVBGPU_NORM_L2 2  /* sqrt(sum x^2)  */
+
+size_t svbgpu_grad_workspace_bytes(uint32_t ntensors);
+
+/* *d_norm = the norm of all elements of all tensors together.  Squares and sums are in 64 bits and the result is
+ * rounded once: large and tiny elements neither overflow nor vanish, and the same tensors give the same bits every
+ * time.  0 without elements; NaN if any element is NaN.  The tensors may overlap (an element counts each time). */
+int svbgpu_grad_norm(int norm, const svbgpu_tensor *tensors, uint32_t ntensors, float *d_norm,
+                     void *d_workspace, size_t workspace_bytes, void *stream);
+
+/* Clips by the global norm N: every element becomes x * c, c = 1 where N + 1e-6 <= max_norm, else
+ * max_norm / (N + 1e-6) (64 bits, rounded once to float32; the product is rounded to float32 and then to the
+ * tensor's type).  N not a number makes every element NaN; N infinite makes c zero.  outs == NULL: in place, and
+ * with c = 1 nothing is written; else tensor i goes to outs[i], of the same type and length, which may be the
+ * tensor itself.  norm_given == 0: N is worked out as by svbgpu_grad_norm and left in *d_norm; norm_given != 0: N is
+ * read from *d_norm (worked out before, or summed over ranks) and neither `norm` nor the workspace is used.
+ * SVBGPU_EINVAL if tensors that are written overlap each other, or one that is read for another. */
+int svbgpu_grad_clip(int norm, const svbgpu_tensor *tensors, uint32_t ntensors, void *const *outs,
+                     double max_norm, int norm_given, float *d_norm, void *d_workspace,
+                     size_t workspace_bytes, void *stream);
+
+/* svbgpu_quantize_encode for gradients, with clipping and error feedback on the way:
+ *   e = g * c + r,  q = (int32) nearest-even(e * scale),  r' = e - q * step,  step = 1 / scale,
+ * the streams of the zigzagged q, and r' for the next step.  Every operation is rounded to float32 by itself.
+ * c is the factor of svbgpu_grad_clip from *d_norm and max_norm (d_norm == NULL: 1).  q saturates at the ends of
+ * int32; an element whose e is infinite or NaN sends 0 and keeps its r.  The receiver calls svbgpu_decode_dequantize
+ * with step.  d_residual_out may be d_residual; otherwise no two buffers overlap.  Bytes of d_out past the stream
+ * are left as they were.  scale and 1 / scale are positive normal numbers.  Workspace as for svbgpu_encode. */
+int svbgpu_quantize_feedback_encode(int variant, int type, const void *d_grad, uint32_t count,
+                                    const float *d_norm, double max_norm, float scale,
+                                    const float *d_residual, float *d_residual_out, uint8_t *d_out,
+                                    void *d_workspace, size_t workspace_bytes, uint64_t *d_written,
+                                    void *stream);
 
 /* Device-pointer form of streamvbyte_compressedbytes / _0124 (reference
  * include/streamvbyte.h:47,55); with SVBGPU_DELTA / SVBGPU_ZIGZAG the size the

@@ -224,6 +224,83 @@ def frame_decode_lists(frames):
     return out[:nv.value], ls
 
 
+# ---- gradient tensors -----------------------------------------------------------
+NORMS = {2: 2, 1: 1, float("inf"): 0}  # norm_type -> SVBGPU_NORM_*
+
+
+def _grad_type(torch, dtype):
+    """SVBGPU_F32 / _F16 / _BF16 of a torch type; ValueError for any other."""
+    types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    if dtype not in types:
+        raise ValueError(f"gradients are float32, float16 or bfloat16, not {dtype}")
+    return types[dtype]
+
+
+def _dense(t):
+    """Whether t's elements fill one stretch of memory, in whatever order."""
+    if t.is_contiguous():
+        return True
+    run = 1
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n > 1), key=lambda x: x[1]):
+        if stride != run:
+            return False
+        run *= size
+    return True
+
+
+class GradSet:
+    """The tensors of one grad_norm / clip_grads call, looked over once and laid out as the C ABI takes them.
+
+    `tensors`: float32, float16 and bfloat16 tensors of one device, mixed as they come, each dense in memory (any
+    order of dimensions).  `out`: tensors of the same types, shapes and strides that clip_grads writes instead.  A program whose
+    gradients keep their memory from step to step makes one GradSet and passes it to every call; it holds the
+    tensors, and raises if one of them has moved since.  Passing a plain list makes one on the spot."""
+
+    def __init__(self, tensors, out=None):
+        import torch
+        from ._lib import GradTensor
+        self.tensors = [t.detach() for t in tensors]  # a later `t.data = ...` of the caller's does not reach these
+        n = len(self.tensors)
+        self.table = (GradTensor * max(n, 1))()
+        self.device = None
+        for i, t in enumerate(self.tensors):
+            self._look(t, f"tensor {i}")
+            self.table[i] = GradTensor(t.data_ptr() or None, t.numel(), _grad_type(torch, t.dtype))
+        self.addresses = [t.data_ptr() for t in self.tensors]
+        self.outs, self.out_table, self.out_addresses = None, None, None
+        if out is not None:
+            self.outs = [t.detach() for t in out]
+            if len(self.outs) != n:
+                raise ValueError(f"{n} tensors, but {len(self.outs)} outputs")
+            for i, (t, y) in enumerate(zip(self.tensors, self.outs)):
+                self._look(y, f"output {i}")
+                same_layout = y.stride() == t.stride() or (y.is_contiguous() and t.is_contiguous())
+                if y.dtype != t.dtype or y.shape != t.shape or not same_layout:
+                    raise ValueError(f"output {i} is not of its tensor's type, shape and strides")
+            self.out_addresses = [t.data_ptr() for t in self.outs]
+            self.out_table = (C.c_void_p * max(n, 1))(*[a or None for a in self.out_addresses])
+
+    def _look(self, t, what):
+        if not t.is_cuda:
+            raise ValueError(f"{what} is not on a device")
+        if self.device is None:
+            self.device = t.device
+        elif t.device != self.device:
+            raise ValueError(f"{what} is on {t.device}, the first on {self.device}")
+        if not _dense(t):
+            raise ValueError(f"{what} has gaps or repeats in its memory: strides {t.stride()} of shape {tuple(t.shape)}")
+
+    def _check(self, device):
+        if self.device is not None and self.device != device:
+            raise ValueError(f"tensors on {self.device}, codec on {device}")
+        if [t.data_ptr() for t in self.tensors] != self.addresses or (
+                self.outs is not None and [t.data_ptr() for t in self.outs] != self.out_addresses):
+            raise ValueError("a tensor of the set has moved since the set was made")
+
+    def __len__(self):
+        return len(self.tensors)
+
+
 class DeviceCodec:
     """Device-pointer API on torch tensors (include/streamvbyte_gpu.h).
 
@@ -238,6 +315,8 @@ class DeviceCodec:
         self.torch = torch
         self.lib = load()
         self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
         with torch.cuda.device(self.device):
             if not self.lib.svbgpu_device_ok():
                 raise SvbError("no usable gfx950 device")
@@ -345,6 +424,82 @@ class DeviceCodec:
                                                      int(accumulate), self.ws.data_ptr(), self.ws_bytes,
                                                      self._res_ptr(1), self._stream()), "svbgpu_decode_dequantize")
         return out, self.res[1:2]
+
+    def _grad_workspace(self, n):
+        need = self.lib.svbgpu_grad_workspace_bytes(n)
+        ws = getattr(self, "_grad_ws", None)
+        if ws is None or ws.numel() < need:
+            ws = self._grad_ws = self.torch.empty(need, dtype=self.torch.uint8, device=self.device)
+        return ws
+
+    def _norm_word(self, t, what):
+        if not (t.device == self.device and t.dtype == self.torch.float32 and t.numel() == 1):
+            raise ValueError(f"{what}: a one-element float32 tensor on {self.device}")
+        return t
+
+    def grad_norm(self, grads, norm_type=2.0, out=None):
+        """Global norm of all elements of `grads` (a GradSet or a list of tensors) -> float32 tensor[1], asynchronously.
+        norm_type 2, 1 or inf.  Sums are in 64 bits, the result is rounded once; the same bits every time."""
+        if norm_type not in NORMS:
+            raise ValueError(f"norm_type {norm_type}: 1, 2 or inf")
+        grads = grads if isinstance(grads, GradSet) else GradSet(grads)
+        grads._check(self.device)
+        norm = self.torch.empty(1, dtype=self.torch.float32, device=self.device) if out is None else self._norm_word(out, "out")
+        ws = self._grad_workspace(len(grads))
+        with self.torch.cuda.device(self.device):
+            _check(self.lib.svbgpu_grad_norm(NORMS[norm_type], grads.table, len(grads), norm.data_ptr(), ws.data_ptr(),
+                                             ws.numel(), self._stream()), "svbgpu_grad_norm")
+        return norm
+
+    def clip_grads(self, grads, max_norm, norm_type=2.0, norm=None):
+        """Multiplies every element of `grads` (a GradSet or a list of tensors) by min(1, max_norm / (N + 1e-6)), N their
+        global norm, in place or into the GradSet's `out` tensors; returns N, a float32 tensor[1].  `norm`: N worked out
+        before (over other ranks' shards too, say); it is then read instead, and returned."""
+        if norm_type not in NORMS:
+            raise ValueError(f"norm_type {norm_type}: 1, 2 or inf")
+        if not max_norm >= 0:
+            raise ValueError(f"max_norm {max_norm}")
+        grads = grads if isinstance(grads, GradSet) else GradSet(grads)
+        grads._check(self.device)
+        given = norm is not None
+        norm = self._norm_word(norm, "norm") if given else self.torch.empty(1, dtype=self.torch.float32, device=self.device)
+        ws = self._grad_workspace(len(grads))
+        with self.torch.cuda.device(self.device):
+            _check(self.lib.svbgpu_grad_clip(NORMS[norm_type], grads.table, len(grads), grads.out_table, max_norm, int(given),
+                                             norm.data_ptr(), ws.data_ptr(), ws.numel(), self._stream()), "svbgpu_grad_clip")
+        return norm
+
+    def quantize_feedback_encode(self, grad, scale, residual, norm=None, max_norm=float("inf"), out=None, residual_out=None,
+                                 variant=V0124):
+        """One gradient tensor (float32, float16 or bfloat16) -> stream of zigzag(q), q = round((grad * c + residual) * scale),
+        with the rest, grad * c + residual - q / scale, left in `residual_out` (default: `residual` itself) for the next
+        step.  c is clip_grads' factor for `norm` and `max_norm` (no norm: 1).  Returns (out_bytes, size_tensor[1],
+        residual_out); the receiver calls decode_dequantize with 1 / scale."""
+        torch = self.torch
+        n = grad.numel()
+        kind = _grad_type(torch, grad.dtype)
+        if n > self.max_count:
+            raise ValueError(f"{n} values, but the codec was made for {self.max_count}")
+        residual_out = residual if residual_out is None else residual_out
+        for t, what in ((grad, "grad"), (residual, "residual"), (residual_out, "residual_out")):
+            if t.device != self.device or not t.is_contiguous() or t.numel() != n:
+                raise ValueError(f"{what}: a contiguous tensor of {n} elements on {self.device}")
+        if residual.dtype != torch.float32 or residual_out.dtype != torch.float32:
+            raise ValueError("the residual is float32")
+        room = streamvbyte_max_compressedbytes(n)
+        if out is None:
+            out = torch.empty(room, dtype=torch.uint8, device=self.device)
+        elif out.device != self.device or out.dtype != torch.uint8 or not out.is_contiguous() or out.numel() < room:
+            raise ValueError(f"out: a contiguous uint8 tensor of at least {room} bytes on {self.device}")
+        if norm is not None:
+            self._norm_word(norm, "norm")
+        with torch.cuda.device(self.device):
+            _check(self.lib.svbgpu_quantize_feedback_encode(variant, kind, grad.data_ptr(), n,
+                                                            None if norm is None else norm.data_ptr(), max_norm, scale,
+                                                            residual.data_ptr(), residual_out.data_ptr(), out.data_ptr(),
+                                                            self.ws.data_ptr(), self.ws_bytes, self._res_ptr(0),
+                                                            self._stream()), "svbgpu_quantize_feedback_encode")
+        return out, self.res[0:1], residual_out
 
     def decode_intersect(self, stream, count, sorted_values, out=None, variant=V1234, prev=0):
         """delta-coded stream x ascending uint32/int32-bits tensor -> (matches buffer, n_matches_tensor[1],

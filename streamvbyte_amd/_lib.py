@@ -14,6 +14,11 @@ class MultiShard(C.Structure):
                 ("d_prev", vp), ("nstreams", C.c_uint32), ("d_sizes_all", vp), ("d_offsets_all", vp)]
 
 
+class GradTensor(C.Structure):
+    """svbgpu_tensor of include/streamvbyte_gpu.h."""
+    _fields_ = [("data", vp), ("count", C.c_uint64), ("type", C.c_int32)]
+
+
 # name -> (restype, argtypes); mirrors include/*.h one to one
 SIGNATURES = {
     # include/streamvbyte.h
@@ -50,6 +55,11 @@ SIGNATURES = {
     "svbgpu_encode": (C.c_int, [C.c_int, C.c_uint, vp, C.c_uint32, vp, C.c_uint32, vp, C.c_size_t, vp, vp]),
     "svbgpu_quantize_encode": (C.c_int, [C.c_int, vp, C.c_uint32, C.c_float, vp, vp, C.c_size_t, vp, vp]),
     "svbgpu_decode_dequantize": (C.c_int, [C.c_int, vp, vp, C.c_uint32, C.c_float, C.c_int, vp, C.c_size_t, vp, vp]),
+    "svbgpu_grad_workspace_bytes": (C.c_size_t, [C.c_uint32]),
+    "svbgpu_grad_norm": (C.c_int, [C.c_int, vp, C.c_uint32, vp, vp, C.c_size_t, vp]),
+    "svbgpu_grad_clip": (C.c_int, [C.c_int, vp, C.c_uint32, vp, C.c_double, C.c_int, vp, vp, C.c_size_t, vp]),
+    "svbgpu_quantize_feedback_encode": (C.c_int, [C.c_int, C.c_int, vp, C.c_uint32, vp, C.c_double, C.c_float, vp, vp,
+                                                  vp, vp, C.c_size_t, vp, vp]),
     "svbgpu_decode_intersect": (C.c_int, [C.c_int, vp, C.c_uint32, C.c_uint32, vp, C.c_uint32, vp, vp, vp, C.c_size_t,
                                           vp, vp]),
     "svbgpu_intersect_workspace_bytes": (C.c_size_t, [C.c_uint32, C.c_uint32]),

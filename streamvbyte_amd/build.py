@@ -2,10 +2,11 @@
 
     python -m streamvbyte_amd.build [--force]
 
-One hipcc invocation over csrc/svb_api.hip; the library lands next to this file
+The translation units of csrc/ side by side, then one link; the library lands next to this file
 so that it travels with the source tree.
 """
 import os
+import re
 import subprocess
 import sys
 
@@ -23,41 +24,59 @@ STRESS_LIB = os.path.join(HERE, "libstreamvbyte_stress.so.2")
 DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
-def sources():
-    out = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC))]
-    out += [os.path.join(ROOT, "include", f) for f in sorted(os.listdir(os.path.join(ROOT, "include")))]
-    return out
+UNITS = ["svb_api", "svb_grad"]  # translation units: csrc/<unit>.hip
+OBJ = os.path.join(HERE, "build")
 
 
-def stale(lib=LIB):
-    if not os.path.exists(lib):
+def with_includes(path, seen=None):
+    """The file and every file of this repository that it includes."""
+    seen = set() if seen is None else seen
+    path = os.path.normpath(path)
+    if path not in seen and os.path.exists(path):
+        seen.add(path)
+        for name in re.findall(r'^#include "([^"]+)"', open(path).read(), flags=re.M):
+            for base in (os.path.dirname(path), os.path.join(ROOT, "include")):
+                with_includes(os.path.join(base, name), seen)
+    return sorted(seen)
+
+
+def stale(out, deps):
+    if not os.path.exists(out):
         return True
-    t = os.path.getmtime(lib)
-    return any(os.path.getmtime(s) > t for s in sources())
+    t = os.path.getmtime(out)
+    return any(os.path.getmtime(s) > t for s in deps)
 
 
-def _compile(out, extra, verbose):
-    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
-           "-Wall", "-Wno-unused-function", *DEVICE_FLAGS, *extra,
-           "-Wl,-soname,libstreamvbyte.so.2",
-           "-I", os.path.join(ROOT, "include"),
-           "-o", out, os.path.join(CSRC, "svb_api.hip"), "-ldl"]
+def _run(cmd, verbose):
     if verbose:
         print(" ".join(cmd), flush=True)
     return subprocess.Popen(cmd)
 
 
+def _wait(jobs):
+    codes = [(j.wait(), j.args) for j in jobs]
+    for rc, args in codes:
+        if rc != 0:
+            raise subprocess.CalledProcessError(rc, args)
+
+
 def build(force=False, verbose=True):
-    """Both libraries, compiled side by side (two hipcc processes)."""
+    """Both libraries: every stale unit compiled side by side, then linked."""
+    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+    os.makedirs(OBJ, exist_ok=True)
+    objects = {LIB: [], STRESS_LIB: []}
     jobs = []
-    if force or stale(LIB):
-        jobs.append(_compile(LIB, [], verbose))
-    if force or stale(STRESS_LIB):
-        jobs.append(_compile(STRESS_LIB, ["-DSVB_LB_STRESS"], verbose))
-    for j in jobs:
-        if j.wait() != 0:
-            raise subprocess.CalledProcessError(j.returncode, j.args)
+    for lib, extra, tag in ((LIB, [], ""), (STRESS_LIB, ["-DSVB_LB_STRESS"], ".stress")):
+        for unit in UNITS:
+            src, obj = os.path.join(CSRC, unit + ".hip"), os.path.join(OBJ, unit + tag + ".o")
+            objects[lib].append(obj)
+            if force or stale(obj, with_includes(src)):
+                jobs.append(_run([hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
+                                  *DEVICE_FLAGS, *extra, "-I", os.path.join(ROOT, "include"), "-c", src, "-o", obj], verbose))
+    _wait(jobs)
+    jobs = [_run([hipcc, "--offload-arch=gfx950", "-fPIC", "-shared", "-Wl,-soname,libstreamvbyte.so.2", "-o", lib, *objs, "-ldl"], verbose)
+            for lib, objs in objects.items() if force or stale(lib, objs)]
+    _wait(jobs)
     if jobs:
         if os.path.lexists(LINK):
             os.remove(LINK)

@@ -25,6 +25,7 @@
 #include "svb_decode.h"
 #include "svb_delta.h"
 #include "svb_encode.h"
+#include "svb_host.h"
 #include "svb_misc.h"
 #include "svb_batch.h"
 #include "svb_lists.h"
@@ -532,6 +533,27 @@ bool bad_flags(unsigned f) { return f & ~(SVBGPU_DELTA | SVBGPU_ZIGZAG); }
 
 }  // namespace
 
+// What the other translation units use of the above (svb_host.h).
+namespace svb {
+namespace host {
+bool device_ok() { return dev_info().ok; }
+int device_cus() { return dev_info().cus; }
+int fail_hip(hipError_t e) {
+  g_last_hip_error = e;
+  return SVBGPU_EHIP;
+}
+int fill_u32(void* ptr, uint32_t value, size_t bytes, hipStream_t st) { return ::fill_u32(ptr, value, bytes, st); }
+int begin_lookback(uint32_t count, void* ws, size_t ws_bytes, hipStream_t st, unsigned* tag2) {
+  const int rc = check_ws(count, ws, ws_bytes);
+  return rc ? rc : prepare_lookback(count, ws, st, tag2);
+}
+int end_lookback(void* ws, hipStream_t st, unsigned tag2) { return finish_lookback(ws, st, tag2); }
+int nt_policy(unsigned long long load_bytes, unsigned long long store_bytes) {
+  return ::nt_policy(options(), load_bytes, store_bytes);
+}
+}  // namespace host
+}  // namespace svb
+
 // =============================================================================
 // Device-pointer API
 // =============================================================================
@@ -546,6 +568,7 @@ const char* svbgpu_strerror(int code) {
     case SVBGPU_EHIP: return hipGetErrorString(g_last_hip_error);
     case SVBGPU_ESCAN: return "device scan gave up waiting on another workgroup";
     case SVBGPU_ETOOBIG: return "count beyond what the library's static scratch is sized for";
+    case SVBGPU_ENOMEM: return "out of host memory";
     default: return "unknown error";
   }
 }
