@@ -265,130 +265,329 @@ __device__ __forceinline__ u32 feed_one(float g, float& r, float c, float scale,
   r = finite ? left : r;
   return (u32)q;
 }
+// A group's four values in the common case, every |q| below 2^22: with w = 2 f + 1/2 (exact), the zigzagged integer is the
+// whole part of |w|, and its width follows from w's exponent: |w| in [1/2, 1) is the integer 0, then every eight
+// exponents are a byte more.  Shifted up by four the exponent's low five bits are at the top; with kWidthBias added the
+// topmost two of them are the code (0124; for 1234 everything below 256 counts as 1 first).  A group is half as many
+// instructions this way as by integers, and the encoder of gradients is short of issue slots, not of bytes.
+template <int V>
+constexpr u32 kWidthBias = V == V0124 ? 9u << 27 : 1u << 27;
+constexpr float kFeedSmall = 4194304.0f;  // 2^22
+template <int V>
+__device__ __forceinline__ u32 feed_group(const float (&g)[4], float (&r)[4], uint4& x, float c, float scale, float step) {
+#pragma clang fp contract(off)
+  float f[4], left[4], w[4];
+  float size = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float e = g[k] * c + r[k];
+    f[k] = rintf(e * scale);
+    left[k] = e - __builtin_fmaf(f[k], step, 0.0f);  // the product; + 0 makes 0 of -0, as the integer would
+    size += fabsf(f[k]);
+    w[k] = __builtin_fmaf(f[k], 2.0f, 0.5f);
+  }
+  if (__ballot(!(size < kFeedSmall)) == 0ull) {  // also false for infinities and NaN
+    u32 key = 0;
+#pragma unroll
+    for (int k = 3; k >= 0; --k) {
+      const float m = V == V1234 ? fmaxf(fabsf(w[k]), 1.0f) : w[k];
+      key = __builtin_amdgcn_alignbit(key, (__float_as_uint(m) << 4) + kWidthBias<V>, 30u);
+      r[k] = left[k];
+    }
+    x = make_uint4((u32)fabsf(w[0]), (u32)fabsf(w[1]), (u32)fabsf(w[2]), (u32)fabsf(w[3]));
+    return key;
+  }
+  u32 z[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) z[k] = zz_enc(feed_one(g[k], r[k], c, scale, step));
+  x = make_uint4(z[0], z[1], z[2], z[3]);
+  return classify_key<V>(x);
+}
 // Four gradients of a group, as they lie in memory.
 template <int T>
 struct Grad4 {
   u32x4_t w;  // float32: four dwords; 16 bits: two
+  template <bool NTL>
   __device__ __forceinline__ void load(const u8* g, u64 first) {
-    if (T == kF32) w = *reinterpret_cast<const u32x4_a4*>(g + 4 * first);
-    else {
-      const u32x2_t h = *reinterpret_cast<const u32x2_a2*>(g + 2 * first);
+    if (T == kF32) {
+      const uint4 t = ld_stream16<NTL>(g + 4 * first);
+      w = u32x4_t{t.x, t.y, t.z, t.w};
+    } else {
+      const u32x2_a2* p = reinterpret_cast<const u32x2_a2*>(g + 2 * first);
+      const u32x2_t h = NTL ? __builtin_nontemporal_load(p) : *p;
       w = u32x4_t{h.x, h.y, 0, 0};
     }
+  }
+  // ... those of them that exist, 0 for the rest
+  __device__ __forceinline__ void load_some(const u8* g, u64 first, u32 count) {
+    w = u32x4_t{0, 0, 0, 0};
+#pragma unroll
+    for (u32 k = 0; k < 4; ++k)
+      if (first + k < count) {
+        if (T == kF32) w[k] = reinterpret_cast<const u32*>(g)[first + k];
+        else w[k >> 1] |= (u32)reinterpret_cast<const unsigned short*>(g)[first + k] << (16 * (k & 1u));
+      }
   }
   __device__ __forceinline__ float get(u32 k) const { return vec_elem<T>(w, k); }
 };
 
-// One pass, tile by tile like k_encode: a workgroup of NW waves draws a tile of NW * QW wave tiles, loads gradients and
-// residuals, quantises, stores the new residuals, finds the tile's place by look-back and assembles its bytes.
-// A wave that runs past the end of the stream takes its groups one element at a time.
-template <int V, int T, int NW, int QW>
-__global__ __launch_bounds__(NW * 64, 4) void k_feedback_encode(const u8* __restrict__ grad, u32 count, u32 n_tiles,
-                                                                u8* __restrict__ out, FeedArgs fa, WsHeader* __restrict__ hdr,
-                                                                LbWords lb, u64* __restrict__ written) {
-  __shared__ EncWaveLds s_lds[NW];
-  __shared__ u32 s_wave_tot[NW];
-  __shared__ u64 s_prefix;
-  __shared__ u32 s_tile;
-  const int lane = lane_id(), wave = wave_id();
-  if (threadIdx.x == 0) s_tile = atomicAdd(&hdr->ticket, 1u);
-  __syncthreads();
-  const u32 tile = __builtin_amdgcn_readfirstlane(s_tile);
-  const u64 keylen = ((u64)count + 3) >> 2;
-  constexpr u64 kTileInts = (u64)NW * QW * kWtInts;
-  const u64 wave_first = (u64)tile * kTileInts + (u64)wave * QW * kWtInts;
-  const float c = fa.norm ? clip_factor(*fa.norm, fa.limit) : 1.0f;
+// Byte counts of a wave tile's groups, scanned: off[j] = bytes before group j*64+lane, total = all of them.
+struct WavePlaces {
+  u32 off[4], total;
+};
+__device__ __forceinline__ WavePlaces wave_places(const u32 (&g)[4], int lane) {
+  // four 16-bit counts in two dwords; a count sums to at most 64 * 16, so none carries into its neighbour
+  const u32 lo = gi_total(g[0]) | (gi_total(g[1]) << 16), hi = gi_total(g[2]) | (gi_total(g[3]) << 16);
+  const u32 inc_lo = wave_scan_incl(lo, lane), inc_hi = wave_scan_incl(hi, lane);
+  const u32 tot_lo = wave_last(inc_lo), tot_hi = wave_last(inc_hi);
+  const u32 ex_lo = inc_lo - lo, ex_hi = inc_hi - hi;
+  const u32 t0 = tot_lo & 0xFFFFu, t1 = tot_lo >> 16, t2 = tot_hi & 0xFFFFu, t3 = tot_hi >> 16;
+  WavePlaces p;
+  p.off[0] = ex_lo & 0xFFFFu;
+  p.off[1] = t0 + (ex_lo >> 16);
+  p.off[2] = t0 + t1 + (ex_hi & 0xFFFFu);
+  p.off[3] = t0 + t1 + t2 + (ex_hi >> 16);
+  p.total = t0 + t1 + t2 + t3;
+  return p;
+}
+// ORs the bytes of a group of at most four bytes into the zeroed image.
+__device__ __forceinline__ void or_small(u8* image, u32 p, u32 L, u32 d) {
+  const u32 sel = shift_selector(p);
+  u32* q = reinterpret_cast<u32*>(image + (p & ~3u));
+  if (L) atomicOr(q, __builtin_amdgcn_perm(d, 0u, sel));
+  if (L + (p & 3u) > 4u) atomicOr(q + 1, __builtin_amdgcn_perm(0u, d, sel));
+}
+// A wave tile's data bytes and keys into the wave's LDS image, from byte 0 of it: where the image goes is not known yet.
+// A quarter in which every value fits a byte -- most quarters of quantised gradients -- needs neither the 64-bit shifts
+// of the general packing nor its five dwords a group.
+template <int V, bool FULL>
+__device__ __forceinline__ void assemble(const uint4 (&x)[4], const u32 (&g)[4], const WavePlaces& p, int lane, EncWaveLds& S) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) S.keys[j * 64 + lane] = (u8)gi_key(g[j]);
+  if (V == V1234) {
+    // plain dword stores, later groups first; see encode_wavetile
+    u32 head[4];
+#pragma unroll
+    for (int j = 3; j >= 0; --j) {
+      const GroupSlot s = group_slot<FULL>(S.data, p.off[j], g[j]);
+      if (FULL && __ballot(gi_key(g[j]) != 0u) == 0ull) {
+        const uint4 d = make_uint4(x[j].x | (x[j].y << 8) | (x[j].z << 16) | (x[j].w << 24), 0, 0, 0);
+        store_dword<0, FULL>(s, d);
+        store_dword<1, FULL>(s, d);
+        head[j] = d.x;
+      } else {
+        const uint4 d = pack_group<V>(x[j], g[j]);
+        store_dword<0, FULL>(s, d);
+        store_dword<1, FULL>(s, d);
+        store_dword<2, FULL>(s, d);
+        store_dword<3, FULL>(s, d);
+        store_dword<4, FULL>(s, d);
+        head[j] = d.x;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) store_head<FULL>(S.data, head[j], p.off[j], g[j]);
+  } else {
+    const u32 nz = (p.total + 15u) >> 4;
+    uint4* l16 = reinterpret_cast<uint4*>(S.data);
+    for (u32 c = lane; c < nz; c += 64) l16[c] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const u32 k = gi_key(g[j]);
+      if (__ballot((k & 0xAAu) != 0u) == 0ull) {  // codes 0 and 1 only
+        u32 d = x[j].w;
+        d = (d << ((k >> 1) & 8u)) | x[j].z;
+        d = (d << ((k << 1) & 8u)) | x[j].y;
+        d = (d << ((k << 3) & 8u)) | x[j].x;
+        or_small(S.data, p.off[j], gi_total(g[j]), d);
+      } else {
+        or_into_image(S.data, p.off[j], gi_total(g[j]), pack_group<V>(x[j], g[j]));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+typedef u32x4_t u32x4_a1 __attribute__((aligned(1)));
+// The image to its place.  The stream starts anywhere, so the 16-byte stores do too.
+template <bool NTS>
+__device__ __forceinline__ void copy_out(const EncWaveLds& S, u32 total, u32 nkeys, int lane, u8* dst, u8* kdst) {
+  const u32x4_t* l16 = reinterpret_cast<const u32x4_t*>(S.data);
+  u32x4_a1* g16 = reinterpret_cast<u32x4_a1*>(dst);
+  const u32 whole = total >> 4;
+  for (u32 c = lane; c < whole; c += 64) {
+    if (NTS) __builtin_nontemporal_store(l16[c], g16 + c);
+    else g16[c] = l16[c];
+  }
+  const u32 rest = 16u * whole + lane;
+  if (rest < total) dst[rest] = S.data[rest];
+  if (4u * lane + 4u <= nkeys) st_u32(kdst + 4 * lane, reinterpret_cast<const u32*>(S.keys)[lane]);
+  else
+    for (u32 b = 4u * lane; b < nkeys; ++b) kdst[b] = S.keys[b];
+}
 
-  uint4 x[QW][4];  // the zigzagged integers
-  u32 lane_tot = 0;
-  const bool full = wave_first + QW * kWtInts <= count;  // wave-uniform
-  if (full) {
+// Values of the group from `first` on that exist, and of a lane's four groups of a wave tile.
+__device__ __forceinline__ u32 present(u64 first, u32 count) { return first < count ? (u32)min((u64)4, (u64)count - first) : 0u; }
+__device__ __forceinline__ u32 present_lane(u64 wt_first, int lane, u32 count) {
+  u32 n = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) n += present(wt_first + (u32)(4 * (j * 64 + lane)), count);
+  return n;
+}
+// One pass.  A workgroup takes tiles off a ticket, QW wave tiles (of 1024 values) for each of its first NW waves; its
+// last wave, the scan wave, draws the tickets and finds the tiles' places by look-back.  A data wave's round:
+//     quantise (values and residuals have arrived), send the new residuals off, count the bytes | barrier A |
+//     assemble the bytes in LDS, request the next tile's values and residuals                  | barrier B | copy out
+// and the scan wave's:
+//     draw the next ticket | A | publish the tile's bytes, look back until the place is known | B |
+// so a tile's look-back runs beside its assembly and the next tile's loads, and the polls never stand in a queue with
+// a data wave's loads and stores.  The barriers order LDS only: __syncthreads would wait for the stores as well.
+// Between a tile's ticket and its publication a workgroup waits only for tiles with smaller tickets: the chain ends.
+//
+// Bound by memory, 12.8 B a value for float32 (0124): 2^26 values in 150 us = 5.7 TB/s; without look-back and tickets
+// (wrong places) the same kernel takes 135 us, and with nothing but the elementwise part 134.  What it took to get
+// there from 187 us, the tile-at-a-time form of k_encode: assembling before the place is known (165), half the
+// instructions a value (feed_group, the one-byte quarters of assemble), one workgroup of 15 data waves per CU instead of
+// two (158; a look-back's answers come slower the more tiles wait) and 30 wave tiles a tile instead of 15 (150).
+template <int V, int T, int NW, int QW, int NT>
+__global__ __launch_bounds__((NW + 1) * 64, 4) void k_feedback_encode(const u8* __restrict__ grad, u32 count, u32 n_tiles,
+                                                                             u8* __restrict__ out, FeedArgs fa,
+                                                                             WsHeader* __restrict__ hdr, LbWords lb,
+                                                                             u64* __restrict__ written) {
+  __shared__ EncWaveLds s_lds[NW * QW];
+  __shared__ u32 s_wave_tot[2][NW];
+  __shared__ u64 s_prefix;
+  __shared__ u32 s_first, s_next;
+  const int lane = lane_id(), wave = wave_id();
+  const u64 keylen = ((u64)count + 3) >> 2;
+  if (wave == NW) {  // the scan wave
+    auto draw = [&]() -> u32 {
+      u32 t = 0;
+      if (lane == 0) t = atomicAdd(&hdr->ticket, 1u);
+      return __builtin_amdgcn_readfirstlane(t);
+    };
+    const bool once = gridDim.x >= n_tiles;  // a workgroup per tile: nobody takes a second one
+    u32 tile = n_tiles > 1 ? draw() : 0u;
+    if (lane == 0) s_first = tile;
+    lds_barrier();
+    if (tile >= n_tiles) return;
+    for (int buf = 0;; buf ^= 1) {
+      const u32 next = once ? n_tiles : draw();
+      if (lane == 0) s_next = next;
+      lds_barrier();  // A
+      const u32 tot = lane < NW ? s_wave_tot[buf][lane] : 0u;
+      const u32 tile_tot = wave_sum(tot);
+      const u64 excl = lb2_exclusive_prefix<2>(lb, tile, tile_tot, lane, &hdr->error);
+      if (lane == 0) {
+        s_prefix = excl;
+        if (tile == n_tiles - 1 && written) *written = keylen + excl + tile_tot;
+        if (tile == 0u) reset_other_ticket(hdr);
+      }
+      lds_barrier();  // B
+      if (next >= n_tiles) return;
+      tile = next;
+    }
+  }
+  const float c = fa.norm ? clip_factor(*fa.norm, fa.limit) : 1.0f;
+  Grad4<T> gr[QW][4];
+  uint4 r[QW][4];
+  auto first_of = [&](u32 tile, int q) -> u64 { return (((u64)tile * NW + wave) * QW + q) * kWtInts; };
+  auto request = [&](u32 tile, int q) {
+    const u64 wt_first = tile < n_tiles ? first_of(tile, q) : count;
+    if (wt_first + kWtInts <= count) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const u64 first = wt_first + (u32)(4 * (j * 64 + lane));
+        gr[q][j].template load<(NT & kNtLoads) != 0>(grad, first);
+        r[q][j] = ld_stream16<(NT & kNtLoads) != 0>(fa.r_in + first);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const u64 first = wt_first + (u32)(4 * (j * 64 + lane));
+        gr[q][j].load_some(grad, first, count);
+        r[q][j] = load_group(reinterpret_cast<const u32*>(fa.r_in), first, count);
+      }
+    }
+  };
+  lds_barrier();
+  u32 tile = __builtin_amdgcn_readfirstlane(s_first);
+  if (tile >= n_tiles) return;
+#pragma unroll
+  for (int q = 0; q < QW; ++q) request(tile, q);
+  for (int buf = 0;; buf ^= 1) {
+    uint4 x[QW][4];  // the zigzagged integers
+    u32 k4[QW];      // their groups' keys
+    u32 lane_tot = 0;
 #pragma unroll
     for (int q = 0; q < QW; ++q) {
-      Grad4<T> g[4];
-      u32x4_t r[4];
+      const u64 wt_first = first_of(tile, q);
+      const bool full = wt_first + kWtInts <= count;  // wave-uniform
+      u32 keys = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const u64 first = wave_first + (u32)(q * kWtInts + 4 * (j * 64 + lane));
-        g[j].load(grad, first);
-        r[j] = *reinterpret_cast<const u32x4_a4*>(fa.r_in + first);
-      }
-      u32 k4 = 0;
+        const float gv[4] = {gr[q][j].get(0), gr[q][j].get(1), gr[q][j].get(2), gr[q][j].get(3)};
+        float rv[4] = {__uint_as_float(r[q][j].x), __uint_as_float(r[q][j].y), __uint_as_float(r[q][j].z), __uint_as_float(r[q][j].w)};
+        u32 key = feed_group<V>(gv, rv, x[q][j], c, fa.scale, fa.step);
+        const u64 first = wt_first + (u32)(4 * (j * 64 + lane));
+        if (full) {
+          st_stream16<(NT & kNtStores) != 0>(fa.r_out + first, make_uint4(__float_as_uint(rv[0]), __float_as_uint(rv[1]),
+                                                                          __float_as_uint(rv[2]), __float_as_uint(rv[3])));
+        } else {
+          const u32 nv = present(first, count);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const u64 first = wave_first + (u32)(q * kWtInts + 4 * (j * 64 + lane));
-        u32 z[4];
-#pragma unroll
-        for (u32 k = 0; k < 4; ++k) {
-          float left = __uint_as_float(r[j][k]);
-          z[k] = zz_enc(feed_one(g[j].get(k), left, c, fa.scale, fa.step));
-          r[j][k] = __float_as_uint(left);
+          for (u32 k = 0; k < 4; ++k)
+            if (k < nv) fa.r_out[first + k] = rv[k];
+          zero_absent(x[q][j], first, count);
+          key &= (1u << (2u * nv)) - 1u;
         }
-        *reinterpret_cast<u32x4_a4*>(fa.r_out + first) = r[j];
-        x[q][j] = make_uint4(z[0], z[1], z[2], z[3]);
-        k4 |= classify_key<V>(x[q][j]) << (8 * j);
+        keys |= key << (8 * j);
       }
-      lane_tot += word_len<V>(k4, 16u);
+      asm volatile("" : "+v"(keys));  // the four keys stay in one register
+      k4[q] = keys;
+      lane_tot += full || V == V0124 ? word_len<V>(keys, 16u) : word_len<V>(keys, present_lane(wt_first, lane, count));
     }
-  } else {
+    const u32 wave_tot = wave_sum(lane_tot);
+    if (lane == 0) s_wave_tot[buf][wave] = wave_tot;
+    lds_barrier();  // A
+    const u32 next = __builtin_amdgcn_readfirstlane(s_next);
+    u32 totals[QW];
 #pragma unroll
-    for (int q = 0; q < QW; ++q)
+    for (int q = 0; q < QW; ++q) {
+      const u64 wt_first = first_of(tile, q);
+      const bool full = wt_first + kWtInts <= count;
+      u32 lens4 = key_lens4<V>(k4[q], 16u);
+      if (!full && V == V1234) {
+        lens4 = code_sums4(k4[q]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const u64 first = wave_first + (u32)(q * kWtInts + 4 * (j * 64 + lane));
-        u32 z[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (u32 k = 0; k < 4; ++k)
-          if (first + k < count) {
-            float left = fa.r_in[first + k];
-            z[k] = zz_enc(feed_one(load_elem<T>(grad, first + k), left, c, fa.scale, fa.step));
-            fa.r_out[first + k] = left;
-          }
-        x[q][j] = make_uint4(z[0], z[1], z[2], z[3]);
-        const u32 nv = first < count ? (u32)min((u64)4, (u64)count - first) : 0u;
-        lane_tot += gi_total(classify_group<V, false>(x[q][j], nv));
+        for (int j = 0; j < 4; ++j) lens4 += present(wt_first + (u32)(4 * (j * 64 + lane)), count) << (8 * j);
       }
-  }
-  const u32 wave_tot = wave_sum(lane_tot);
-  if (lane == 0) s_wave_tot[wave] = wave_tot;
-  __syncthreads();
-  if (wave == 0) {
-    u32 tile_tot = 0;
+      u32 g[4];  // the groups' descriptors
 #pragma unroll
-    for (int w = 0; w < NW; ++w) tile_tot += s_wave_tot[w];
-    const u64 excl = lb2_exclusive_prefix<2>(lb, tile, tile_tot, lane, &hdr->error);
-    if (lane == 0) {
-      s_prefix = excl;
-      if (tile == n_tiles - 1 && written) *written = keylen + excl + tile_tot;
-      if (tile == 0u) reset_other_ticket(hdr);
+      for (int j = 0; j < 4; ++j) g[j] = ((k4[q] >> (8 * j)) & 0xFFu) | (((lens4 >> (8 * j)) & 0xFFu) << 24);
+      const WavePlaces places = wave_places(g, lane);
+      totals[q] = places.total;
+      if (full) assemble<V, true>(x[q], g, places, lane, s_lds[wave * QW + q]);
+      else assemble<V, false>(x[q], g, places, lane, s_lds[wave * QW + q]);
+      __builtin_amdgcn_sched_barrier(0);
+      request(next, q);
+      __builtin_amdgcn_sched_barrier(0);
     }
-  }
-  __syncthreads();
-  u64 doff = s_prefix;
-  for (int w = 0; w < wave; ++w) doff += s_wave_tot[w];
-  EncWaveLds& S = s_lds[wave];
-  u8* data_out = out + keylen;
-#pragma unroll 1
-  for (int q = 0; q < QW; ++q) {
-    const u64 wt_first = wave_first + (u64)q * kWtInts;
-    u32 g[4];
-    if (full) {
+    lds_barrier();  // B
+    u64 doff = keylen + s_prefix;
+    for (int w = 0; w < wave; ++w) doff += s_wave_tot[buf][w];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) g[j] = classify_group<V, true>(x[0][j], 4u);
-      doff += encode_wavetile<V, true>(x[0], g, kWtInts, lane, S, data_out + doff, out + (wt_first >> 2));
-    } else if (wt_first < count) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const u64 first = wt_first + 4u * (j * 64 + lane);
-        g[j] = classify_group<V, false>(x[0][j], first < count ? (u32)min((u64)4, (u64)count - first) : 0u);
-      }
-      const u32 nints = (u32)min((u64)kWtInts, (u64)count - wt_first);
-      doff += encode_wavetile<V, false>(x[0], g, nints, lane, S, data_out + doff, out + (wt_first >> 2));
+    for (int q = 0; q < QW; ++q) {
+      const u64 wt_first = first_of(tile, q);
+      if (wt_first < count)
+        copy_out<(NT & kNtStores) != 0>(s_lds[wave * QW + q], totals[q], (u32)((min((u64)kWtInts, (u64)count - wt_first) + 3) >> 2), lane,
+                                        out + doff, out + (wt_first >> 2));
+      doff += totals[q];
     }
-#pragma unroll
-    for (int r = 0; r + 1 < QW; ++r)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[r][j] = x[r + 1][j];
+    if (next >= n_tiles) return;
+    tile = next;
   }
 }
 

@@ -133,16 +133,31 @@ int norm_of(int kind, const svbgpu_tensor* t, uint32_t n, u64 total, float* d_no
   return run_norm<kNormEuclid>(t, n, total, d_norm, partial, st);
 }
 
+template <int V, int T, int NW, int QW, int NT>
+void launch_feedback(const void* grad, uint32_t count, uint8_t* d_out, const FeedArgs& fa, void* ws, unsigned tag2, uint64_t* d_written,
+                     hipStream_t st) {
+  static_assert(NW * QW >= kWaves, "ws_layout has room for a look-back word per kWaves wave tiles");
+  const WsLayout L = ws_layout(count);
+  constexpr u32 kTile = NW * QW * kWtInts;
+  const u32 tiles = (u32)(((u64)count + kTile - 1) / kTile);
+  const u32 grid = std::min<u32>(tiles, (u32)std::max(host::device_cus(), 1));
+  WsHeader* h = reinterpret_cast<WsHeader*>(static_cast<char*>(ws) + ((tag2 >> 3) & 1u) * 8);
+  const LbWords lb{reinterpret_cast<u64*>(static_cast<char*>(ws) + L.off_status), (u32)((L.off_lb_group - L.off_status) / 8), tag2};
+  hipLaunchKernelGGL((k_feedback_encode<V, T, NW, QW, NT>), dim3(grid), dim3((NW + 1) * 64), 0, st, static_cast<const u8*>(grad), count,
+                     tiles, d_out, fa, h, lb, d_written);
+}
+// The tile by size: large tiles have fewer look-backs, small ones spread a short stream over the device.  Measured
+// (float32, 0124; us at 2^16 / 2^20 / 2^22 / 2^23 / 2^24 / 2^26 values): 7 wave tiles 5.8 / 8.8 / 23 / 40 / 69 / 217,
+// 15: 7.4 / 8.7 / 17 / 26 / 50 / 163, 30: 12 / 13 / 16 / 28 / 49 / 151.  Non-temporal stores and loads from the sizes at
+// which what a call touches no longer stays in the Infinity Cache (2^23: stores 30 -> 26, loads too 30; 2^26: 161 -> 156 ->
+// 151).
 template <int V, int T>
 void launch_feedback(const void* grad, uint32_t count, uint8_t* d_out, const FeedArgs& fa, void* ws, unsigned tag2, uint64_t* d_written,
                      hipStream_t st) {
-  constexpr int NW = 8, QW = 2;
-  const WsLayout L = ws_layout(count);
-  const u32 tiles = (u32)(((u64)count + NW * QW * kWtInts - 1) / (NW * QW * kWtInts));
-  WsHeader* h = reinterpret_cast<WsHeader*>(static_cast<char*>(ws) + ((tag2 >> 3) & 1u) * 8);
-  const LbWords lb{reinterpret_cast<u64*>(static_cast<char*>(ws) + L.off_status), (u32)((L.off_lb_group - L.off_status) / 8), tag2};
-  hipLaunchKernelGGL((k_feedback_encode<V, T, NW, QW>), dim3(tiles), dim3(NW * 64), 0, st, static_cast<const u8*>(grad), count, tiles,
-                     d_out, fa, h, lb, d_written);
+  if (count < (1u << 20)) launch_feedback<V, T, 7, 1, 0>(grad, count, d_out, fa, ws, tag2, d_written, st);
+  else if (count < (1u << 23)) launch_feedback<V, T, 15, 1, 0>(grad, count, d_out, fa, ws, tag2, d_written, st);
+  else if (count < (1u << 24)) launch_feedback<V, T, 15, 1, kNtStores>(grad, count, d_out, fa, ws, tag2, d_written, st);
+  else launch_feedback<V, T, 15, 2, kNtLoads | kNtStores>(grad, count, d_out, fa, ws, tag2, d_written, st);
 }
 
 }  // namespace
