@@ -436,7 +436,8 @@ __device__ __forceinline__ u32 present_lane(u64 wt_first, int lane, u32 count) {
   for (int j = 0; j < 4; ++j) n += present(wt_first + (u32)(4 * (j * 64 + lane)), count);
   return n;
 }
-// One pass.  A workgroup takes tiles off a ticket, QW wave tiles (of 1024 values) for each of its first NW waves; its
+constexpr u32 kFeedMaxWaves = 15;  // data waves of a workgroup, at most
+// One pass.  A workgroup takes tiles off a ticket, QW wave tiles (of 1024 values) for each of its first nw waves; its
 // last wave, the scan wave, draws the tickets and finds the tiles' places by look-back.  A data wave's round:
 //     quantise (values and residuals have arrived), send the new residuals off, count the bytes | barrier A |
 //     assemble the bytes in LDS, request the next tile's values and residuals                  | barrier B | copy out
@@ -451,18 +452,18 @@ __device__ __forceinline__ u32 present_lane(u64 wt_first, int lane, u32 count) {
 // there from 187 us, the tile-at-a-time form of k_encode: assembling before the place is known (165), half the
 // instructions a value (feed_group, the one-byte quarters of assemble), one workgroup of 15 data waves per CU instead of
 // two (158; a look-back's answers come slower the more tiles wait) and 30 wave tiles a tile instead of 15 (150).
-template <int V, int T, int NW, int QW, int NT>
-__global__ __launch_bounds__((NW + 1) * 64, 4) void k_feedback_encode(const u8* __restrict__ grad, u32 count, u32 n_tiles,
+template <int V, int T, int QW, int NT>
+__global__ __launch_bounds__(kFeedMaxWaves * 64 + 64, 4) void k_feedback_encode(const u8* __restrict__ grad, u32 count, u32 n_tiles, u32 nw,
                                                                              u8* __restrict__ out, FeedArgs fa,
                                                                              WsHeader* __restrict__ hdr, LbWords lb,
                                                                              u64* __restrict__ written) {
-  __shared__ EncWaveLds s_lds[NW * QW];
-  __shared__ u32 s_wave_tot[2][NW];
+  __shared__ EncWaveLds s_lds[kFeedMaxWaves * QW];
+  __shared__ u32 s_wave_tot[2][kFeedMaxWaves];
   __shared__ u64 s_prefix;
   __shared__ u32 s_first, s_next;
   const int lane = lane_id(), wave = wave_id();
   const u64 keylen = ((u64)count + 3) >> 2;
-  if (wave == NW) {  // the scan wave
+  if (wave == (int)nw) {  // the scan wave
     auto draw = [&]() -> u32 {
       u32 t = 0;
       if (lane == 0) t = atomicAdd(&hdr->ticket, 1u);
@@ -477,7 +478,7 @@ __global__ __launch_bounds__((NW + 1) * 64, 4) void k_feedback_encode(const u8* 
       const u32 next = once ? n_tiles : draw();
       if (lane == 0) s_next = next;
       lds_barrier();  // A
-      const u32 tot = lane < NW ? s_wave_tot[buf][lane] : 0u;
+      const u32 tot = lane < (int)nw ? s_wave_tot[buf][lane] : 0u;
       const u32 tile_tot = wave_sum(tot);
       const u64 excl = lb2_exclusive_prefix<2>(lb, tile, tile_tot, lane, &hdr->error);
       if (lane == 0) {
@@ -493,7 +494,7 @@ __global__ __launch_bounds__((NW + 1) * 64, 4) void k_feedback_encode(const u8* 
   const float c = fa.norm ? clip_factor(*fa.norm, fa.limit) : 1.0f;
   Grad4<T> gr[QW][4];
   uint4 r[QW][4];
-  auto first_of = [&](u32 tile, int q) -> u64 { return (((u64)tile * NW + wave) * QW + q) * kWtInts; };
+  auto first_of = [&](u32 tile, int q) -> u64 { return (((u64)tile * nw + wave) * QW + q) * kWtInts; };
   auto request = [&](u32 tile, int q) {
     const u64 wt_first = tile < n_tiles ? first_of(tile, q) : count;
     if (wt_first + kWtInts <= count) {

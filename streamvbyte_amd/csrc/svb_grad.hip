@@ -133,31 +133,34 @@ int norm_of(int kind, const svbgpu_tensor* t, uint32_t n, u64 total, float* d_no
   return run_norm<kNormEuclid>(t, n, total, d_norm, partial, st);
 }
 
-template <int V, int T, int NW, int QW, int NT>
-void launch_feedback(const void* grad, uint32_t count, uint8_t* d_out, const FeedArgs& fa, void* ws, unsigned tag2, uint64_t* d_written,
-                     hipStream_t st) {
-  static_assert(NW * QW >= kWaves, "ws_layout has room for a look-back word per kWaves wave tiles");
-  const WsLayout L = ws_layout(count);
-  constexpr u32 kTile = NW * QW * kWtInts;
-  const u32 tiles = (u32)(((u64)count + kTile - 1) / kTile);
+template <int V, int T, int QW, int NT>
+void launch_feedback(u32 nw, const void* grad, uint32_t count, uint8_t* d_out, const FeedArgs& fa, void* ws, unsigned tag2,
+                     uint64_t* d_written, hipStream_t st) {
+  const WsLayout L = ws_layout(count);  // has a look-back word per kWaves wave tiles: nw * QW >= kWaves
+  const u32 tile = nw * QW * kWtInts, tiles = (u32)(((u64)count + tile - 1) / tile);
   const u32 grid = std::min<u32>(tiles, (u32)std::max(host::device_cus(), 1));
   WsHeader* h = reinterpret_cast<WsHeader*>(static_cast<char*>(ws) + ((tag2 >> 3) & 1u) * 8);
   const LbWords lb{reinterpret_cast<u64*>(static_cast<char*>(ws) + L.off_status), (u32)((L.off_lb_group - L.off_status) / 8), tag2};
-  hipLaunchKernelGGL((k_feedback_encode<V, T, NW, QW, NT>), dim3(grid), dim3((NW + 1) * 64), 0, st, static_cast<const u8*>(grad), count,
-                     tiles, d_out, fa, h, lb, d_written);
+  hipLaunchKernelGGL((k_feedback_encode<V, T, QW, NT>), dim3(grid), dim3((nw + 1) * 64), 0, st, static_cast<const u8*>(grad), count,
+                     tiles, nw, d_out, fa, h, lb, d_written);
 }
-// The tile by size: large tiles have fewer look-backs, small ones spread a short stream over the device.  Measured
-// (float32, 0124; us at 2^16 / 2^20 / 2^22 / 2^23 / 2^24 / 2^26 values): 7 wave tiles 5.8 / 8.8 / 23 / 40 / 69 / 217,
-// 15: 7.4 / 8.7 / 17 / 26 / 50 / 163, 30: 12 / 13 / 16 / 28 / 49 / 151.  Non-temporal stores and loads from the sizes at
-// which what a call touches no longer stays in the Infinity Cache (2^23: stores 30 -> 26, loads too 30; 2^26: 161 -> 156 ->
-// 151).
+// The tile by size.  A large tile means few look-backs, a small one that a short stream reaches more of the device and
+// that the last round of workgroups is fuller.  Measured with float32, 0124, us for QW x nw wave tiles a tile:
+//     2^18 values: 1x4 6.3, 1x8 6.7, 1x15 7.9                2^20: 1x4 10.4, 1x8 8.6, 1x15 9.0, 2x15 12.7
+//     3 * 2^20: 1x8 17.5, 1x15 13.4, 2x15 14.9               2^22: 1x15 17.4, 2x15 16.5
+//     6 * 2^20: 1x15 23.6, 2x15 19.8                         2^24: 1x15 49.3, 2x11 48.0, 2x15 50.9
+//     2^25: 1x15 86.7, 2x11 82.7, 2x15 83.9
+// Non-temporal stores from 2^23 values up and loads from 2^24, where what a call touches no longer stays in the Infinity
+// Cache (2^23: 30 us, with such stores 26, with the loads too 30; 2^26: 161, 156, 151).
 template <int V, int T>
 void launch_feedback(const void* grad, uint32_t count, uint8_t* d_out, const FeedArgs& fa, void* ws, unsigned tag2, uint64_t* d_written,
                      hipStream_t st) {
-  if (count < (1u << 20)) launch_feedback<V, T, 7, 1, 0>(grad, count, d_out, fa, ws, tag2, d_written, st);
-  else if (count < (1u << 23)) launch_feedback<V, T, 15, 1, 0>(grad, count, d_out, fa, ws, tag2, d_written, st);
-  else if (count < (1u << 24)) launch_feedback<V, T, 15, 1, kNtStores>(grad, count, d_out, fa, ws, tag2, d_written, st);
-  else launch_feedback<V, T, 15, 2, kNtLoads | kNtStores>(grad, count, d_out, fa, ws, tag2, d_written, st);
+  const u32 m = count >> 19;  // in half millions
+  if (m < 4) launch_feedback<V, T, 1, 0>(m < 1 ? 4 : 8, grad, count, d_out, fa, ws, tag2, d_written, st);
+  else if (m < 7) launch_feedback<V, T, 1, 0>(15, grad, count, d_out, fa, ws, tag2, d_written, st);
+  else if (m < 16) launch_feedback<V, T, 2, 0>(15, grad, count, d_out, fa, ws, tag2, d_written, st);
+  else if (m < 32) launch_feedback<V, T, 1, kNtStores>(15, grad, count, d_out, fa, ws, tag2, d_written, st);
+  else launch_feedback<V, T, 2, kNtLoads | kNtStores>(11, grad, count, d_out, fa, ws, tag2, d_written, st);
 }
 
 }  // namespace
