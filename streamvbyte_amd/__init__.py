@@ -259,26 +259,33 @@ class GradSet:
     def __init__(self, tensors, out=None):
         import torch
         from ._lib import GradTensor
-        self.tensors = [t.detach() for t in tensors]  # a later `t.data = ...` of the caller's does not reach these
-        n = len(self.tensors)
-        self.table = (GradTensor * max(n, 1))()
+        tensors = [t.detach() for t in tensors]  # a later `t.data = ...` of the caller's does not reach these
+        outs = None if out is None else [t.detach() for t in out]
         self.device = None
-        for i, t in enumerate(self.tensors):
+        for i, t in enumerate(tensors):
             self._look(t, f"tensor {i}")
-            self.table[i] = GradTensor(t.data_ptr() or None, t.numel(), _grad_type(torch, t.dtype))
-        self.addresses = [t.data_ptr() for t in self.tensors]
-        self.outs, self.out_table, self.out_addresses = None, None, None
-        if out is not None:
-            self.outs = [t.detach() for t in out]
-            if len(self.outs) != n:
-                raise ValueError(f"{n} tensors, but {len(self.outs)} outputs")
-            for i, (t, y) in enumerate(zip(self.tensors, self.outs)):
+        if outs is not None:
+            if len(outs) != len(tensors):
+                raise ValueError(f"{len(tensors)} tensors, but {len(outs)} outputs")
+            for i, (t, y) in enumerate(zip(tensors, outs)):
                 self._look(y, f"output {i}")
                 same_layout = y.stride() == t.stride() or (y.is_contiguous() and t.is_contiguous())
                 if y.dtype != t.dtype or y.shape != t.shape or not same_layout:
                     raise ValueError(f"output {i} is not of its tensor's type, shape and strides")
-            self.out_addresses = [t.data_ptr() for t in self.outs]
-            self.out_table = (C.c_void_p * max(n, 1))(*[a or None for a in self.out_addresses])
+        # in the order of the memory that a clip writes, in which the library checks it fastest
+        written = tensors if outs is None else outs
+        order = sorted(range(len(tensors)), key=lambda i: written[i].data_ptr())
+        self.tensors = [tensors[i] for i in order]
+        self.outs = None if outs is None else [outs[i] for i in order]
+        n = len(tensors)
+        self.table = (GradTensor * max(n, 1))(*[GradTensor(t.data_ptr() or None, t.numel(), _grad_type(torch, t.dtype))
+                                                for t in self.tensors])
+        self.out_table = None if outs is None else (C.c_void_p * max(n, 1))(*[t.data_ptr() or None for t in self.outs])
+        # a tensor keeps its place in its storage, so one tensor a storage tells whether any has moved
+        self._held = list({t.untyped_storage().data_ptr(): t for t in self.tensors + (self.outs or [])}.values())
+        self._addresses = [t.data_ptr() for t in self._held]
+        self._indices = list(range(len(self._held)))
+        self._compare = getattr(torch._C, "_tensors_data_ptrs_at_indices_equal", None)
 
     def _look(self, t, what):
         if not t.is_cuda:
@@ -293,8 +300,11 @@ class GradSet:
     def _check(self, device):
         if self.device is not None and self.device != device:
             raise ValueError(f"tensors on {self.device}, codec on {device}")
-        if [t.data_ptr() for t in self.tensors] != self.addresses or (
-                self.outs is not None and [t.data_ptr() for t in self.outs] != self.out_addresses):
+        if self._compare is not None:  # torch's own comparison, twice as fast as a loop
+            same = self._compare(self._held, self._addresses, self._indices)
+        else:
+            same = [t.data_ptr() for t in self._held] == self._addresses
+        if not same:
             raise ValueError("a tensor of the set has moved since the set was made")
 
     def __len__(self):
@@ -425,6 +435,19 @@ class DeviceCodec:
                                                      self._res_ptr(1), self._stream()), "svbgpu_decode_dequantize")
         return out, self.res[1:2]
 
+    def _call(self, what, *args):
+        """lib.<what>(*args, stream) on torch's current stream of the codec's device, checked."""
+        torch = self.torch
+        index = self.device.index
+        args += (torch._C._cuda_getCurrentRawStream(index),)
+        if torch._C._cuda_getDevice() == index:
+            rc = getattr(self.lib, what)(*args)
+        else:
+            with torch.cuda.device(index):
+                rc = getattr(self.lib, what)(*args)
+        if rc:
+            _check(rc, what)
+
     def _grad_workspace(self, n):
         need = self.lib.svbgpu_grad_workspace_bytes(n)
         ws = getattr(self, "_grad_ws", None)
@@ -446,9 +469,7 @@ class DeviceCodec:
         grads._check(self.device)
         norm = self.torch.empty(1, dtype=self.torch.float32, device=self.device) if out is None else self._norm_word(out, "out")
         ws = self._grad_workspace(len(grads))
-        with self.torch.cuda.device(self.device):
-            _check(self.lib.svbgpu_grad_norm(NORMS[norm_type], grads.table, len(grads), norm.data_ptr(), ws.data_ptr(),
-                                             ws.numel(), self._stream()), "svbgpu_grad_norm")
+        self._call("svbgpu_grad_norm", NORMS[norm_type], grads.table, len(grads), norm.data_ptr(), ws.data_ptr(), ws.numel())
         return norm
 
     def clip_grads(self, grads, max_norm, norm_type=2.0, norm=None):
@@ -464,9 +485,8 @@ class DeviceCodec:
         given = norm is not None
         norm = self._norm_word(norm, "norm") if given else self.torch.empty(1, dtype=self.torch.float32, device=self.device)
         ws = self._grad_workspace(len(grads))
-        with self.torch.cuda.device(self.device):
-            _check(self.lib.svbgpu_grad_clip(NORMS[norm_type], grads.table, len(grads), grads.out_table, max_norm, int(given),
-                                             norm.data_ptr(), ws.data_ptr(), ws.numel(), self._stream()), "svbgpu_grad_clip")
+        self._call("svbgpu_grad_clip", NORMS[norm_type], grads.table, len(grads), grads.out_table, max_norm, int(given),
+                   norm.data_ptr(), ws.data_ptr(), ws.numel())
         return norm
 
     def quantize_feedback_encode(self, grad, scale, residual, norm=None, max_norm=float("inf"), out=None, residual_out=None,
@@ -493,12 +513,9 @@ class DeviceCodec:
             raise ValueError(f"out: a contiguous uint8 tensor of at least {room} bytes on {self.device}")
         if norm is not None:
             self._norm_word(norm, "norm")
-        with torch.cuda.device(self.device):
-            _check(self.lib.svbgpu_quantize_feedback_encode(variant, kind, grad.data_ptr(), n,
-                                                            None if norm is None else norm.data_ptr(), max_norm, scale,
-                                                            residual.data_ptr(), residual_out.data_ptr(), out.data_ptr(),
-                                                            self.ws.data_ptr(), self.ws_bytes, self._res_ptr(0),
-                                                            self._stream()), "svbgpu_quantize_feedback_encode")
+        self._call("svbgpu_quantize_feedback_encode", variant, kind, grad.data_ptr(), n, None if norm is None else norm.data_ptr(),
+                   max_norm, scale, residual.data_ptr(), residual_out.data_ptr(), out.data_ptr(), self.ws.data_ptr(),
+                   self.ws_bytes, self._res_ptr(0))
         return out, self.res[0:1], residual_out
 
     def decode_intersect(self, stream, count, sorted_values, out=None, variant=V1234, prev=0):

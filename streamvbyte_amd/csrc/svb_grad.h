@@ -69,51 +69,55 @@ __device__ __forceinline__ u32x4_t scale_vec(const u32x4_t& v, float c) {
 
 // ---- tables of tensors ----------------------------------------------------------------------------------
 // A launch carries its tensors in its arguments (4 KiB at most), so nothing is copied to the device, nothing is kept
-// there, and a captured launch holds all it needs.  Every tensor is cut into chunks of `chunk_bytes`; a workgroup
-// takes one, and finds the tensor it belongs to by a binary search on the first chunks.
+// there, and a captured launch holds all it needs.  Every tensor is cut into chunks of `chunk_bytes`; a workgroup (or,
+// for small sets, a wave) takes one at a time.
 struct GradSpan {
   u64 addr;   // bits 57..56 the type, below them the address
   u64 where;  // bits 63..40 the launch's index of the tensor's first chunk, below them its elements
 };
-constexpr u32 kMaxSpans = 240;       // spans of a launch without outputs
-constexpr u32 kMaxSpansOut = 160;    // ... and with an output address each
 constexpr int kAddrBits = 56, kCountBits = 40;
+constexpr u32 kMaxSpans = 240;     // spans of a launch without outputs
+constexpr u32 kMaxSpansOut = 160;  // ... with an output address each
+constexpr u32 kMaxSpansSmall = 64; // ... of the one-workgroup kernel
 template <u32 N>
 struct GradTable {
   GradSpan span[N];
   u32 n;
-  u32 chunk_bytes;  // a multiple of kGradStep vectors
+  u32 chunk_bytes;  // a multiple of 16
+  u32 chunks;
 };
 template <u32 N>
 struct GradOuts {
   u64 addr[N];
 };
-constexpr u32 kGradThreads = 256;
-constexpr u32 kGradUnroll = 8;                              // 16-byte loads a lane has in flight
-constexpr u32 kGradStep = kGradThreads * kGradUnroll;       // vectors of one round of a workgroup
-constexpr u32 kGradMinChunk = 2 * 16 * kGradStep;           // 64 KiB
-
 struct GradChunk {
+  u64 addr;   // of its first element
+  u64 skip;   // bytes of the tensor before it
   u32 span;
   int type;
-  u64 first;  // first element in the tensor
   u32 count;  // elements
 };
+// The chunk's tensor is the last span that starts at or before it.  Every lane looks at a few spans and the ballots are
+// counted: one trip to the arguments, where a binary search takes eight that wait for each other.
 template <u32 N>
 __device__ __forceinline__ GradChunk find_chunk(const GradTable<N>& t, u32 chunk) {
-  u32 lo = 0, hi = t.n;  // span[lo] starts at or before the chunk, span[hi] after it
-  while (hi - lo > 1) {
-    const u32 mid = (lo + hi) >> 1;
-    if ((u32)(t.span[mid].where >> kCountBits) <= chunk) lo = mid;
-    else hi = mid;
+  const u32 lane = lane_id();
+  u32 before = 0;
+#pragma unroll
+  for (u32 i = 0; i < (N + 63) / 64; ++i) {
+    const u32 k = i * 64 + lane;
+    const bool starts = k < t.n && (u32)(t.span[min(k, N - 1)].where >> kCountBits) <= chunk;
+    before += (u32)__popcll(__ballot(starts));
   }
-  const u64 where = t.span[lo].where;
   GradChunk c;
-  c.span = lo;
-  c.type = (int)(t.span[lo].addr >> kAddrBits);
-  const u32 elems = c.type == kF32 ? t.chunk_bytes >> 2 : t.chunk_bytes >> 1;
-  c.first = (u64)(chunk - (u32)(where >> kCountBits)) * elems;
-  c.count = (u32)min((u64)elems, (where & ((1ull << kCountBits) - 1)) - c.first);
+  c.span = __builtin_amdgcn_readfirstlane(before) - 1;  // span 0 starts at chunk 0
+  const GradSpan s = t.span[c.span];
+  c.type = (int)(s.addr >> kAddrBits);
+  const u32 shift = c.type == kF32 ? 2u : 1u, elems = t.chunk_bytes >> shift;
+  const u64 first = (u64)(chunk - (u32)(s.where >> kCountBits)) * elems;
+  c.count = (u32)min((u64)elems, (s.where & ((1ull << kCountBits) - 1)) - first);
+  c.skip = first << shift;
+  c.addr = (s.addr & ((1ull << kAddrBits) - 1)) + c.skip;
   return c;
 }
 
@@ -123,7 +127,7 @@ __device__ __forceinline__ GradChunk find_chunk(const GradTable<N>& t, u32 chunk
 // at the end.  The maximum is taken on the bits of |x|, where NaN stands above everything.
 template <int KIND>
 struct NormSum {
-  double s0 = 0.0, s1 = 0.0;
+  double s0 = 0.0, s1 = 0.0;  // two chains of additions
   u32 m = 0;
   __device__ __forceinline__ void add(float x, bool odd) {
     if (KIND == kNormMax) m = max(m, __float_as_uint(x) & 0x7FFFFFFFu);
@@ -134,9 +138,15 @@ struct NormSum {
     }
   }
 };
-// Combination over the workgroup, the same in every run; result in thread 0.
+// What a chunk, a workgroup or the whole set comes to: the bits of a double, or those of a float32 maximum.
 template <int KIND>
-__device__ __forceinline__ u64 norm_block(double s, u32 m, u64* s_tmp, u32 waves) {
+__device__ __forceinline__ u64 norm_join(u64 a, u64 b) {
+  if (KIND == kNormMax) return max(a, b);
+  return (u64)__double_as_longlong(__longlong_as_double((long long)a) + __longlong_as_double((long long)b));
+}
+// Combination over the workgroup, the same in every run; result in every thread.
+template <int KIND, u32 WAVES>
+__device__ __forceinline__ u64 norm_block(double s, u32 m, u64* s_tmp) {
   if (KIND == kNormMax) {
 #pragma unroll
     for (int d = 32; d; d >>= 1) m = max(m, (u32)__shfl_xor((int)m, d));
@@ -146,58 +156,74 @@ __device__ __forceinline__ u64 norm_block(double s, u32 m, u64* s_tmp, u32 waves
   }
   if (lane_id() == 0) s_tmp[wave_id()] = KIND == kNormMax ? (u64)m : (u64)__double_as_longlong(s);
   __syncthreads();
-  u64 r = s_tmp[0];
-  for (u32 w = 1; w < waves; ++w)
-    r = KIND == kNormMax ? max(r, s_tmp[w])
-                         : (u64)__double_as_longlong(__longlong_as_double((long long)r) + __longlong_as_double((long long)s_tmp[w]));
-  return r;
-}
-template <int KIND, int T>
-__device__ __forceinline__ void norm_chunk(const u8* p, u32 count, NormSum<KIND>& acc) {
-  const u32 nv = count / kVecElems<T>;
-  const u32x4_a2* v = reinterpret_cast<const u32x4_a2*>(p);
-  for (u32 base = threadIdx.x; base < nv; base += kGradStep) {
-    u32x4_t x[kGradUnroll];
+  u64 r[WAVES];
 #pragma unroll
-    for (u32 i = 0; i < kGradUnroll; ++i) {
+  for (u32 w = 0; w < WAVES; ++w) r[w] = s_tmp[w];
+#pragma unroll
+  for (u32 w = 1; w < WAVES; w <<= 1)
+#pragma unroll
+    for (u32 i = 0; i + w < WAVES; i += 2 * w) r[i] = norm_join<KIND>(r[i], r[i + w]);
+  return r[0];
+}
+template <int KIND>
+__device__ __forceinline__ float norm_value(u64 r) {
+  if (KIND == kNormMax) return __uint_as_float((u32)r);
+  const double total = __longlong_as_double((long long)r);
+  return (float)(KIND == kNormEuclid ? sqrt(total) : total);
+}
+// A chunk by THREADS threads, of which this is number `id`, with UNROLL 16-byte loads in flight each.
+template <int KIND, int T, bool NTL, u32 THREADS, u32 UNROLL>
+__device__ __forceinline__ void norm_chunk(u64 addr, u32 count, u32 id, NormSum<KIND>& acc) {
+  const u32 nv = count / kVecElems<T>;
+  const u32x4_a2* v = reinterpret_cast<const u32x4_a2*>(addr);
+  for (u32 base = id; base < nv; base += THREADS * UNROLL) {
+    u32x4_t x[UNROLL];
+#pragma unroll
+    for (u32 i = 0; i < UNROLL; ++i) {
       x[i] = u32x4_t{0, 0, 0, 0};
-      if (base + i * kGradThreads < nv) x[i] = v[base + i * kGradThreads];
+      if (base + i * THREADS < nv) x[i] = NTL ? __builtin_nontemporal_load(v + base + i * THREADS) : v[base + i * THREADS];
     }
 #pragma unroll
-    for (u32 i = 0; i < kGradUnroll; ++i)
+    for (u32 i = 0; i < UNROLL; ++i)
 #pragma unroll
       for (u32 k = 0; k < kVecElems<T>; ++k) acc.add(vec_elem<T>(x[i], k), k & 1u);
   }
-  const u32 rest = nv * kVecElems<T> + threadIdx.x;
-  if (rest < count) acc.add(load_elem<T>(p, rest), false);
+  const u32 rest = nv * kVecElems<T> + id;
+  if (rest < count) acc.add(load_elem<T>(reinterpret_cast<const u8*>(addr), rest), false);
 }
+template <int KIND, bool NTL, u32 THREADS, u32 UNROLL>
+__device__ __forceinline__ void norm_any(const GradChunk& c, u32 id, NormSum<KIND>& acc) {
+  if (c.type == kF32) norm_chunk<KIND, kF32, NTL, THREADS, UNROLL>(c.addr, c.count, id, acc);
+  else if (c.type == kF16) norm_chunk<KIND, kF16, NTL, THREADS, UNROLL>(c.addr, c.count, id, acc);
+  else norm_chunk<KIND, kBF16, NTL, THREADS, UNROLL>(c.addr, c.count, id, acc);
+}
+// The chunks' sums.  Bound by memory: 2^28 float32 in 155 us = 6.9 TB/s, with k_grad_finish 160.  The loads are
+// non-temporal (181 us without): what is read once and is larger than the caches only turns them over.  The last chunks
+// of a clip's norm, from `nt_chunks` on, are read to stay, for k_grad_scale begins with them.
+constexpr u32 kNormThreads = 256, kNormUnroll = 8;
 template <int KIND>
-__global__ __launch_bounds__(kGradThreads) void k_grad_norm(GradTable<kMaxSpans> t, u64* __restrict__ partial) {
-  __shared__ u64 s_tmp[kGradThreads / 64];
+__global__ __launch_bounds__(kNormThreads) void k_grad_norm(GradTable<kMaxSpans> t, u64* __restrict__ partial, u32 nt_chunks) {
+  __shared__ u64 s_tmp[kNormThreads / 64];
   const GradChunk c = find_chunk(t, blockIdx.x);
-  const u8* p = reinterpret_cast<const u8*>(t.span[c.span].addr & ((1ull << kAddrBits) - 1)) + c.first * (c.type == kF32 ? 4u : 2u);
   NormSum<KIND> acc;
-  if (c.type == kF32) norm_chunk<KIND, kF32>(p, c.count, acc);
-  else if (c.type == kF16) norm_chunk<KIND, kF16>(p, c.count, acc);
-  else norm_chunk<KIND, kBF16>(p, c.count, acc);
-  const u64 r = norm_block<KIND>(acc.s0 + acc.s1, acc.m, s_tmp, kGradThreads / 64);
+  if (blockIdx.x < nt_chunks) norm_any<KIND, true, kNormThreads, kNormUnroll>(c, threadIdx.x, acc);
+  else norm_any<KIND, false, kNormThreads, kNormUnroll>(c, threadIdx.x, acc);
+  const u64 r = norm_block<KIND, kNormThreads / 64>(acc.s0 + acc.s1, acc.m, s_tmp);
   if (threadIdx.x == 0) partial[blockIdx.x] = r;
 }
-// The chunks' sums to the norm: one workgroup.
+// The chunks' sums to the norm: one workgroup, four loads of a thread in flight.
 template <int KIND>
 __global__ __launch_bounds__(1024) void k_grad_finish(const u64* __restrict__ partial, u32 n, float* __restrict__ norm) {
   __shared__ u64 s_tmp[16];
-  double s = 0.0;
-  u32 m = 0;
-  for (u32 i = threadIdx.x; i < n; i += 1024) {
-    if (KIND == kNormMax) m = max(m, (u32)partial[i]);
-    else s += __longlong_as_double((long long)partial[i]);
+  u64 s = 0;  // the bits of 0.0 as well
+  for (u32 i = threadIdx.x; i < n; i += 4 * 1024) {
+    u64 p[4];
+#pragma unroll
+    for (u32 k = 0; k < 4; ++k) p[k] = i + 1024 * k < n ? partial[i + 1024 * k] : 0;
+    s = norm_join<KIND>(s, norm_join<KIND>(norm_join<KIND>(p[0], p[1]), norm_join<KIND>(p[2], p[3])));
   }
-  const u64 r = norm_block<KIND>(s, m, s_tmp, 16);
-  if (threadIdx.x == 0) {
-    const double total = __longlong_as_double((long long)r);
-    *norm = KIND == kNormMax ? __uint_as_float((u32)r) : (float)(KIND == kNormEuclid ? sqrt(total) : total);
-  }
+  const u64 r = norm_block<KIND, 16>(__longlong_as_double((long long)s), (u32)s, s_tmp);
+  if (threadIdx.x == 0) *norm = norm_value<KIND>(r);
 }
 
 // ---- clipping ----------------------------------------------------------------------------------------------
@@ -207,38 +233,68 @@ __device__ __forceinline__ float clip_factor(float norm, double limit) {
   const double n = (double)norm + kNormEps;
   return n <= limit ? 1.0f : (float)(limit / n);
 }
-template <int T>
-__device__ __forceinline__ void scale_chunk(const u8* p, u8* q, u32 count, float c) {
+template <int T, bool NT, u32 THREADS, u32 UNROLL>
+__device__ __forceinline__ void scale_chunk(u64 from, u64 to, u32 count, u32 id, float c) {
   const u32 nv = count / kVecElems<T>;
-  const u32x4_a2* v = reinterpret_cast<const u32x4_a2*>(p);
-  u32x4_a2* w = reinterpret_cast<u32x4_a2*>(q);
-  for (u32 base = threadIdx.x; base < nv; base += kGradStep) {
-    u32x4_t x[kGradUnroll];
+  const u32x4_a2* v = reinterpret_cast<const u32x4_a2*>(from);
+  u32x4_a2* w = reinterpret_cast<u32x4_a2*>(to);
+  for (u32 base = id; base < nv; base += THREADS * UNROLL) {
+    u32x4_t x[UNROLL];
 #pragma unroll
-    for (u32 i = 0; i < kGradUnroll; ++i)
-      if (base + i * kGradThreads < nv) x[i] = v[base + i * kGradThreads];
+    for (u32 i = 0; i < UNROLL; ++i)
+      if (base + i * THREADS < nv) x[i] = NT ? __builtin_nontemporal_load(v + base + i * THREADS) : v[base + i * THREADS];
 #pragma unroll
-    for (u32 i = 0; i < kGradUnroll; ++i)
-      if (base + i * kGradThreads < nv) w[base + i * kGradThreads] = scale_vec<T>(x[i], c);
+    for (u32 i = 0; i < UNROLL; ++i)
+      if (base + i * THREADS < nv) {
+        const u32x4_t y = scale_vec<T>(x[i], c);
+        if (NT) __builtin_nontemporal_store(y, w + base + i * THREADS);
+        else w[base + i * THREADS] = y;
+      }
   }
-  const u32 rest = nv * kVecElems<T> + threadIdx.x;
-  if (rest < count) store_elem<T>(q, rest, __fmul_rn(load_elem<T>(p, rest), c));
+  const u32 rest = nv * kVecElems<T> + id;
+  if (rest < count)
+    store_elem<T>(reinterpret_cast<u8*>(to), rest, __fmul_rn(load_elem<T>(reinterpret_cast<const u8*>(from), rest), c));
 }
-// y = x * factor, rounded to the tensor's type; in place unless `outs` says otherwise, and then a factor of 1 leaves
-// nothing to do.
-template <bool OUT>
-__global__ __launch_bounds__(kGradThreads) void k_grad_scale(GradTable<kMaxSpansOut> t, GradOuts<kMaxSpansOut> outs,
-                                                             const float* __restrict__ norm, double limit) {
+template <bool NT, u32 THREADS, u32 UNROLL>
+__device__ __forceinline__ void scale_any(const GradChunk& c, u64 to, u32 id, float f) {
+  if (c.type == kF32) scale_chunk<kF32, NT, THREADS, UNROLL>(c.addr, to, c.count, id, f);
+  else if (c.type == kF16) scale_chunk<kF16, NT, THREADS, UNROLL>(c.addr, to, c.count, id, f);
+  else scale_chunk<kBF16, NT, THREADS, UNROLL>(c.addr, to, c.count, id, f);
+}
+// y = x * factor, rounded to the tensor's type; in place unless OUT, and then a factor of 1 leaves nothing to do.  The
+// chunks are taken last first: the end of what the norm has just read is still in the Infinity Cache.  Bound by memory,
+// read and write: 2^28 float32 in 340 us = 6.3 TB/s.  Small chunks and non-temporal accesses, so that the workgroups in
+// flight cover one compact stretch and what is written does not turn the cache over (385 us with chunks of 128 KiB, in
+// order and with plain accesses).
+constexpr u32 kScaleThreads = 256, kScaleUnroll = 4, kScaleChunk = 16 * kScaleThreads * kScaleUnroll;
+template <bool OUT, bool NT>
+__global__ __launch_bounds__(kScaleThreads) void k_grad_scale(GradTable<kMaxSpansOut> t, GradOuts<kMaxSpansOut> outs,
+                                                              const float* __restrict__ norm, double limit) {
   const float f = clip_factor(*norm, limit);
   if (!OUT && f == 1.0f) return;
-  const GradChunk c = find_chunk(t, blockIdx.x);
-  const u64 skip = c.first * (c.type == kF32 ? 4u : 2u);
-  const u64 from = t.span[c.span].addr & ((1ull << kAddrBits) - 1);
-  const u8* p = reinterpret_cast<const u8*>(from) + skip;
-  u8* q = reinterpret_cast<u8*>(OUT ? outs.addr[c.span] : from) + skip;
-  if (c.type == kF32) scale_chunk<kF32>(p, q, c.count, f);
-  else if (c.type == kF16) scale_chunk<kF16>(p, q, c.count, f);
-  else scale_chunk<kBF16>(p, q, c.count, f);
+  const GradChunk c = find_chunk(t, gridDim.x - 1 - blockIdx.x);
+  scale_any<NT, kScaleThreads, kScaleUnroll>(c, OUT ? outs.addr[c.span] + c.skip : c.addr, threadIdx.x, f);
+}
+
+// A small set in one launch of one workgroup: chunk by chunk to the waves, the norm, and for a clip the chunks again.
+// A launch and its place in the queue cost more than the bytes: a handful of small tensors takes 3 us this way, 6 by
+// k_grad_norm and k_grad_finish.
+constexpr u32 kSmallChunk = 4096, kSmallChunks = 64;  // bytes; chunks at most
+template <int KIND, bool CLIP, bool OUT>
+__global__ __launch_bounds__(1024) void k_grad_small(GradTable<kMaxSpansSmall> t, GradOuts<kMaxSpansSmall> outs,
+                                                     float* __restrict__ norm, double limit) {
+  __shared__ u64 s_tmp[16];
+  NormSum<KIND> acc;
+  for (u32 i = wave_id(); i < t.chunks; i += 16) norm_any<KIND, false, 64, 4>(find_chunk(t, i), lane_id(), acc);
+  const float n = norm_value<KIND>(norm_block<KIND, 16>(acc.s0 + acc.s1, acc.m, s_tmp));  // its barrier: all is read
+  if (threadIdx.x == 0) *norm = n;
+  if (!CLIP) return;
+  const float f = clip_factor(n, limit);
+  if (!OUT && f == 1.0f) return;
+  for (u32 i = wave_id(); i < t.chunks; i += 16) {
+    const GradChunk c = find_chunk(t, i);
+    scale_any<false, 64, 4>(c, OUT ? outs.addr[c.span] + c.skip : c.addr, lane_id(), f);
+  }
 }
 
 // ---- quantise with feedback, then encode -----------------------------------------------------------------

@@ -23,8 +23,10 @@ namespace {
 
 inline hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
-constexpr u32 kGradChunks = 8192;      // chunks of one call, apart from one a tensor
-constexpr u32 kMaxTensors = 1u << 22;  // so that a chunk's index fits 24 bits
+constexpr u64 kCacheBytes = 256ull << 20;  // Infinity Cache
+constexpr u32 kNormMinChunk = 64 << 10;   // bytes of a norm's chunk ...
+constexpr u32 kNormChunks = 4096;         // ... which grows so that there are no more than this many, and one a tensor
+constexpr u32 kMaxTensors = 1u << 22;     // so that a chunk's index in its launch fits 24 bits
 
 bool bad_type(int t) { return t != SVBGPU_F32 && t != SVBGPU_F16 && t != SVBGPU_BF16; }
 bool bad_norm(int n) { return n != SVBGPU_NORM_MAX && n != SVBGPU_NORM_L1 && n != SVBGPU_NORM_L2; }
@@ -52,7 +54,6 @@ int check_tensors(const svbgpu_tensor* t, uint32_t n, u64* total) {
 
 struct Range {
   u64 begin, end;
-  uint32_t index;
 };
 bool by_begin(const Range& a, const Range& b) { return a.begin < b.begin; }
 // No memory that a clip writes may be written twice, or read for another tensor than its own.
@@ -67,70 +68,136 @@ int check_written(const svbgpu_tensor* t, uint32_t n, void* const* outs) {
     const u64 begin = (u64)(uintptr_t)(outs ? outs[i] : t[i].data), bytes = t[i].count * elem_bytes(t[i].type);
     if (!begin || (begin & (elem_bytes(t[i].type) - 1)) || begin >> kAddrBits) { fine = false; break; }
     if (m && begin < r[m - 1].begin) sorted = false;
-    r[m++] = Range{begin, begin + bytes, i};
+    r[m++] = Range{begin, begin + bytes};
   }
   if (fine && !sorted) std::sort(r, r + m, by_begin);
   for (uint32_t i = 1; fine && i < m; ++i) fine = r[i - 1].end <= r[i].begin;
-  for (uint32_t i = 0; fine && outs && i < n; ++i) {  // an input may meet its own output, exactly, and no other
-    if (!t[i].count || outs[i] == t[i].data) continue;
-    const u64 begin = (u64)(uintptr_t)t[i].data, end = begin + t[i].count * elem_bytes(t[i].type);
-    const Range* after = std::lower_bound(r, r + m, Range{end, 0, 0}, by_begin);  // the first that starts at or after the end
-    fine = after == r || after[-1].end <= begin;
+  if (fine && outs) {  // neighbours in memory are one range from here on: the views of a bucket come down to the bucket
+    uint32_t k = 0;
+    for (uint32_t i = 1; i < m; ++i) {
+      if (r[i].begin == r[k].end) r[k].end = r[i].end;
+      else r[++k] = r[i];
+    }
+    m = m ? k + 1 : 0;
+    for (uint32_t i = 0; fine && i < n; ++i) {  // an input may meet its own output, exactly, and no other
+      if (!t[i].count || outs[i] == t[i].data) continue;
+      const u64 begin = (u64)(uintptr_t)t[i].data, end = begin + t[i].count * elem_bytes(t[i].type);
+      const Range* after = std::lower_bound(r, r + m, Range{end, 0}, by_begin);  // the first that starts at or after the end
+      fine = after == r || after[-1].end <= begin;
+    }
   }
   if (r != on_stack) delete[] r;
   return fine ? SVBGPU_OK : SVBGPU_EINVAL;
 }
 
-u32 chunk_bytes_of(u64 total) {
-  u64 c = kGradMinChunk;
-  while (c * kGradChunks < total) c <<= 1;
-  return (u32)std::min<u64>(c, 1u << 31);
+u32 chunks_of(const svbgpu_tensor& t, u32 chunk_bytes) {
+  const u64 elems = chunk_bytes / elem_bytes(t.type);
+  return (u32)((t.count + elems - 1) / elems);
 }
-
-// Cuts the tensors into launches of at most N spans; launch(table, first tensor of span 0.., chunks, chunks before).
-template <u32 N, class F>
-int for_launches(const svbgpu_tensor* t, uint32_t n, u32 chunk_bytes, F launch) {
-  GradTable<N> table;
-  uint32_t of_span[N];
-  u32 before = 0, chunks = 0;
-  table.n = 0;
-  table.chunk_bytes = chunk_bytes;
-  for (uint32_t i = 0; i <= n; ++i) {
-    if (table.n == N || (i == n && table.n)) {
-      const int rc = launch(table, of_span, chunks, before);
-      if (rc) return rc;
-      before += chunks;
-      chunks = 0;
-      table.n = 0;
+// Appends a tensor to a launch's table.
+template <u32 N>
+void append(GradTable<N>& table, const svbgpu_tensor& t) {
+  table.span[table.n++] = GradSpan{(u64)(uintptr_t)t.data | ((u64)t.type << kAddrBits), ((u64)table.chunks << kCountBits) | t.count};
+  table.chunks += chunks_of(t, table.chunk_bytes);
+}
+// Chunks small enough for a wave and few enough for one workgroup?
+bool is_small(const svbgpu_tensor* t, uint32_t n, u64 total) {
+  if (total > (u64)kSmallChunk * kSmallChunks) return false;
+  u32 chunks = 0, spans = 0;
+  for (uint32_t i = 0; i < n; ++i)
+    if (t[i].count) {
+      chunks += chunks_of(t[i], kSmallChunk);
+      if (++spans > kMaxSpansSmall || chunks > kSmallChunks) return false;
     }
-    if (i == n || !t[i].count) continue;
-    table.span[table.n] = GradSpan{(u64)(uintptr_t)t[i].data | ((u64)t[i].type << kAddrBits), ((u64)chunks << kCountBits) | t[i].count};
-    of_span[table.n++] = i;
-    const u64 elems = chunk_bytes / elem_bytes(t[i].type);
-    chunks += (u32)((t[i].count + elems - 1) / elems);
-  }
-  return SVBGPU_OK;
+  return true;
 }
 
 template <int KIND>
-int run_norm(const svbgpu_tensor* t, uint32_t n, u64 total, float* d_norm, u64* partial, hipStream_t st) {
-  u32 chunks_all = 0;
-  const int rc = for_launches<kMaxSpans>(t, n, chunk_bytes_of(total), [&](const GradTable<kMaxSpans>& table, const uint32_t*, u32 chunks, u32 before) {
-    hipLaunchKernelGGL(k_grad_norm<KIND>, dim3(chunks), dim3(kGradThreads), 0, st, table, partial + before);
-    GRAD_HIP(hipGetLastError());
-    chunks_all = before + chunks;
-    return SVBGPU_OK;
-  });
-  if (rc) return rc;
-  hipLaunchKernelGGL(k_grad_finish<KIND>, dim3(1), dim3(1024), 0, st, partial, chunks_all, d_norm);
+int launch_small(const svbgpu_tensor* t, uint32_t n, void* const* outs, bool clip, float* d_norm, double limit, hipStream_t st) {
+  GradTable<kMaxSpansSmall> table;
+  GradOuts<kMaxSpansSmall> o;
+  table.n = table.chunks = 0;
+  table.chunk_bytes = kSmallChunk;
+  for (uint32_t i = 0; i < n; ++i)
+    if (t[i].count) {
+      o.addr[table.n] = outs ? (u64)(uintptr_t)outs[i] : 0;
+      append(table, t[i]);
+    }
+  if (!clip) hipLaunchKernelGGL((k_grad_small<KIND, false, false>), dim3(1), dim3(1024), 0, st, table, o, d_norm, limit);
+  else if (outs) hipLaunchKernelGGL((k_grad_small<KIND, true, true>), dim3(1), dim3(1024), 0, st, table, o, d_norm, limit);
+  else hipLaunchKernelGGL((k_grad_small<KIND, true, false>), dim3(1), dim3(1024), 0, st, table, o, d_norm, limit);
   GRAD_HIP(hipGetLastError());
   return SVBGPU_OK;
 }
-int norm_of(int kind, const svbgpu_tensor* t, uint32_t n, u64 total, float* d_norm, void* ws, hipStream_t st) {
-  u64* partial = static_cast<u64*>(ws);
-  if (kind == SVBGPU_NORM_MAX) return run_norm<kNormMax>(t, n, total, d_norm, partial, st);
-  if (kind == SVBGPU_NORM_L1) return run_norm<kNormSum>(t, n, total, d_norm, partial, st);
-  return run_norm<kNormEuclid>(t, n, total, d_norm, partial, st);
+// keep: bytes at the end of the set that are read to stay in the cache.
+template <int KIND>
+int launch_norm(const svbgpu_tensor* t, uint32_t n, u64 total, u64 keep, float* d_norm, u64* partial, hipStream_t st) {
+  u64 chunk = kNormMinChunk;
+  while (chunk * kNormChunks < total) chunk <<= 1;
+  GradTable<kMaxSpans> table;
+  table.chunk_bytes = (u32)std::min<u64>(chunk, 1u << 31);
+  const u64 passing = total > keep ? total - keep : 0;  // bytes read to pass
+  u64 bytes = 0;                                        // ... of the set that earlier launches read
+  u32 before = 0;                                       // chunks of earlier launches
+  for (uint32_t i = 0; i < n;) {
+    u64 mine = 0;
+    table.n = table.chunks = 0;
+    for (; i < n && table.n < kMaxSpans; ++i)
+      if (t[i].count) {
+        append(table, t[i]);
+        mine += t[i].count * elem_bytes(t[i].type);
+      }
+    if (!table.n) break;
+    const u32 nt = passing <= bytes ? 0 : passing >= bytes + mine ? table.chunks : (u32)((double)(passing - bytes) / (double)mine * table.chunks);
+    hipLaunchKernelGGL(k_grad_norm<KIND>, dim3(table.chunks), dim3(kNormThreads), 0, st, table, partial + before, nt);
+    GRAD_HIP(hipGetLastError());
+    before += table.chunks;
+    bytes += mine;
+  }
+  hipLaunchKernelGGL(k_grad_finish<KIND>, dim3(1), dim3(1024), 0, st, partial, before, d_norm);
+  GRAD_HIP(hipGetLastError());
+  return SVBGPU_OK;
+}
+// y = x * factor, the last tensors first.
+int launch_scale(const svbgpu_tensor* t, uint32_t n, u64 total, void* const* outs, const float* d_norm, double limit, hipStream_t st) {
+  const bool nt = (host::nt_policy(total, total) & kNtStores) != 0;
+  GradTable<kMaxSpansOut> table;
+  GradOuts<kMaxSpansOut> o;
+  uint32_t of_span[kMaxSpansOut];
+  table.chunk_bytes = kScaleChunk;
+  while ((u64)table.chunk_bytes << 23 < total) table.chunk_bytes <<= 1;  // the chunks' index has 24 bits
+  for (uint32_t i = n; i;) {
+    u32 k = 0;
+    for (; i && k < kMaxSpansOut; --i)
+      if (t[i - 1].count) of_span[k++] = i - 1;
+    if (!k) break;
+    table.n = table.chunks = 0;
+    while (k--) {  // in the set's order, which the kernel takes from the end
+      o.addr[table.n] = outs ? (u64)(uintptr_t)outs[of_span[k]] : 0;
+      append(table, t[of_span[k]]);
+    }
+    const dim3 grid(table.chunks), block(kScaleThreads);
+    if (outs && nt) hipLaunchKernelGGL((k_grad_scale<true, true>), grid, block, 0, st, table, o, d_norm, limit);
+    else if (outs) hipLaunchKernelGGL((k_grad_scale<true, false>), grid, block, 0, st, table, o, d_norm, limit);
+    else if (nt) hipLaunchKernelGGL((k_grad_scale<false, true>), grid, block, 0, st, table, o, d_norm, limit);
+    else hipLaunchKernelGGL((k_grad_scale<false, false>), grid, block, 0, st, table, o, d_norm, limit);
+    GRAD_HIP(hipGetLastError());
+  }
+  return SVBGPU_OK;
+}
+template <int KIND>
+int run_kind(const svbgpu_tensor* t, uint32_t n, u64 total, void* const* outs, bool clip, double limit, float* d_norm, void* ws,
+             hipStream_t st) {
+  if (is_small(t, n, total)) return launch_small<KIND>(t, n, outs, clip, d_norm, limit, st);
+  const u64 keep = clip ? kCacheBytes : (host::nt_policy(total, 0) & kNtLoads) ? 0 : total;
+  const int rc = launch_norm<KIND>(t, n, total, keep, d_norm, static_cast<u64*>(ws), st);
+  return rc || !clip ? rc : launch_scale(t, n, total, outs, d_norm, limit, st);
+}
+int run(int kind, const svbgpu_tensor* t, uint32_t n, u64 total, void* const* outs, bool clip, double limit, float* d_norm, void* ws,
+        hipStream_t st) {
+  if (kind == SVBGPU_NORM_MAX) return run_kind<kNormMax>(t, n, total, outs, clip, limit, d_norm, ws, st);
+  if (kind == SVBGPU_NORM_L1) return run_kind<kNormSum>(t, n, total, outs, clip, limit, d_norm, ws, st);
+  return run_kind<kNormEuclid>(t, n, total, outs, clip, limit, d_norm, ws, st);
 }
 
 template <int V, int T, int QW, int NT>
@@ -167,7 +234,7 @@ void launch_feedback(const void* grad, uint32_t count, uint8_t* d_out, const Fee
 
 extern "C" {
 
-size_t svbgpu_grad_workspace_bytes(uint32_t ntensors) { return align256(8 * ((size_t)kGradChunks + ntensors)); }
+size_t svbgpu_grad_workspace_bytes(uint32_t ntensors) { return align256(8 * ((size_t)kNormChunks + ntensors)); }
 
 int svbgpu_grad_norm(int norm, const svbgpu_tensor* tensors, uint32_t ntensors, float* d_norm, void* ws, size_t ws_bytes, void* stream) {
   u64 total;
@@ -176,7 +243,7 @@ int svbgpu_grad_norm(int norm, const svbgpu_tensor* tensors, uint32_t ntensors, 
   if (rc) return rc;
   if (!ws || ((uintptr_t)ws & 255u) || ws_bytes < svbgpu_grad_workspace_bytes(ntensors)) return SVBGPU_EWORKSPACE;
   if (!host::device_ok()) return SVBGPU_ENODEVICE;
-  return norm_of(norm, tensors, ntensors, total, d_norm, ws, S(stream));
+  return run(norm, tensors, ntensors, total, nullptr, false, 0.0, d_norm, ws, S(stream));
 }
 
 int svbgpu_grad_clip(int norm, const svbgpu_tensor* tensors, uint32_t ntensors, void* const* outs, double max_norm, int norm_given,
@@ -188,20 +255,8 @@ int svbgpu_grad_clip(int norm, const svbgpu_tensor* tensors, uint32_t ntensors, 
   if (rc) return rc;
   if (!norm_given && (!ws || ((uintptr_t)ws & 255u) || ws_bytes < svbgpu_grad_workspace_bytes(ntensors))) return SVBGPU_EWORKSPACE;
   if (!host::device_ok()) return SVBGPU_ENODEVICE;
-  hipStream_t st = S(stream);
-  if (!norm_given) {
-    rc = norm_of(norm, tensors, ntensors, total, d_norm, ws, st);
-    if (rc) return rc;
-  }
-  return for_launches<kMaxSpansOut>(tensors, ntensors, chunk_bytes_of(total),
-                                    [&](const GradTable<kMaxSpansOut>& table, const uint32_t* of_span, u32 chunks, u32) {
-    GradOuts<kMaxSpansOut> o;
-    for (u32 i = 0; i < table.n; ++i) o.addr[i] = outs ? (u64)(uintptr_t)outs[of_span[i]] : 0;
-    if (outs) hipLaunchKernelGGL(k_grad_scale<true>, dim3(chunks), dim3(kGradThreads), 0, st, table, o, d_norm, max_norm);
-    else hipLaunchKernelGGL(k_grad_scale<false>, dim3(chunks), dim3(kGradThreads), 0, st, table, o, d_norm, max_norm);
-    GRAD_HIP(hipGetLastError());
-    return SVBGPU_OK;
-  });
+  if (norm_given) return launch_scale(tensors, ntensors, total, outs, d_norm, max_norm, S(stream));
+  return run(norm, tensors, ntensors, total, outs, true, max_norm, d_norm, ws, S(stream));
 }
 
 int svbgpu_quantize_feedback_encode(int variant, int type, const void* d_grad, uint32_t count, const float* d_norm, double max_norm,
