@@ -289,14 +289,14 @@ int svbgpu_grad_norm(int norm, const svbgpu_tensor *tensors, uint32_t ntensors, 
  * with c = 1 nothing is written; else tensor i goes to outs[i], of the same type and length, which may be the
  * tensor itself.  norm_given == 0: N is worked out as by svbgpu_grad_norm and left in *d_norm; norm_given != 0: N is
  * read from *d_norm (worked out before, or summed over ranks) and neither `norm` nor the workspace is used.
- * SVBGPU_EINVAL if tensors that are written overlap each other, or one that is read for another. */
+ * SVBGPU_EINVAL if tensors that are written overlap each other, or one that is read for another, or the norm. */
 int svbgpu_grad_clip(int norm, const svbgpu_tensor *tensors, uint32_t ntensors, void *const *outs,
                      double max_norm, int norm_given, float *d_norm, void *d_workspace,
                      size_t workspace_bytes, void *stream);
 
 /* svbgpu_quantize_encode for gradients, with clipping and error feedback on the way:
- *   e = g * c + r,  q = (int32) nearest-even(e * scale),  r' = e - q * step,  step = 1 / scale,
- * the streams of the zigzagged q, and r' for the next step.  Every operation is rounded to float32 by itself.
+ *   e = g * c + r,  q = (int32) nearest-even(e * scale),  r' = e - q * step,  step = 1.0f / scale,
+ * the stream of the zigzagged q, and r' for the next step.  Every operation is rounded to float32 by itself.
  * c is the factor of svbgpu_grad_clip from *d_norm and max_norm (d_norm == NULL: 1).  q saturates at the ends of
  * int32; an element whose e is infinite or NaN sends 0 and keeps its r.  The receiver calls svbgpu_decode_dequantize
  * with step.  d_residual_out may be d_residual; otherwise no two buffers overlap.  Bytes of d_out past the stream

@@ -288,8 +288,8 @@ class GradSet:
         self._compare = getattr(torch._C, "_tensors_data_ptrs_at_indices_equal", None)
 
     def _look(self, t, what):
-        if not t.is_cuda:
-            raise ValueError(f"{what} is not on a device")
+        if not t.is_cuda or str(t.layout) != "torch.strided":
+            raise ValueError(f"{what} is not a dense tensor on a device")
         if self.device is None:
             self.device = t.device
         elif t.device != self.device:
@@ -449,11 +449,14 @@ class DeviceCodec:
             _check(rc, what)
 
     def _grad_workspace(self, n):
+        """A workspace for n tensors.  One that was handed out is never freed: a captured graph may hold its address."""
         need = self.lib.svbgpu_grad_workspace_bytes(n)
-        ws = getattr(self, "_grad_ws", None)
-        if ws is None or ws.numel() < need:
-            ws = self._grad_ws = self.torch.empty(need, dtype=self.torch.uint8, device=self.device)
-        return ws
+        kept = self.__dict__.setdefault("_grad_ws", [])
+        if not kept or kept[-1].numel() < need:
+            if kept:
+                need = max(need, 2 * kept[-1].numel())
+            kept.append(self.torch.empty(need, dtype=self.torch.uint8, device=self.device))
+        return kept[-1]
 
     def _norm_word(self, t, what):
         if not (t.device == self.device and t.dtype == self.torch.float32 and t.numel() == 1):
@@ -462,7 +465,8 @@ class DeviceCodec:
 
     def grad_norm(self, grads, norm_type=2.0, out=None):
         """Global norm of all elements of `grads` (a GradSet or a list of tensors) -> float32 tensor[1], asynchronously.
-        norm_type 2, 1 or inf.  Sums are in 64 bits, the result is rounded once; the same bits every time."""
+        norm_type 2, 1 or inf.  Sums are in 64 bits, the result is rounded once; the same bits every time.  Calls of one
+        codec share its workspaces: they, and replays of graphs that hold them, are ordered on one stream."""
         if norm_type not in NORMS:
             raise ValueError(f"norm_type {norm_type}: 1, 2 or inf")
         grads = grads if isinstance(grads, GradSet) else GradSet(grads)
@@ -492,9 +496,9 @@ class DeviceCodec:
     def quantize_feedback_encode(self, grad, scale, residual, norm=None, max_norm=float("inf"), out=None, residual_out=None,
                                  variant=V0124):
         """One gradient tensor (float32, float16 or bfloat16) -> stream of zigzag(q), q = round((grad * c + residual) * scale),
-        with the rest, grad * c + residual - q / scale, left in `residual_out` (default: `residual` itself) for the next
-        step.  c is clip_grads' factor for `norm` and `max_norm` (no norm: 1).  Returns (out_bytes, size_tensor[1],
-        residual_out); the receiver calls decode_dequantize with 1 / scale."""
+        with the rest, grad * c + residual - q * step, left in `residual_out` (default: `residual` itself) for the next
+        step.  c is clip_grads' factor for `norm` and `max_norm` (no norm: 1); step is float32(1) / float32(scale), what the
+        receiver gives to decode_dequantize.  Returns (out_bytes, size_tensor[1], residual_out)."""
         torch = self.torch
         n = grad.numel()
         kind = _grad_type(torch, grad.dtype)

@@ -253,6 +253,10 @@ int svbgpu_grad_clip(int norm, const svbgpu_tensor* tensors, uint32_t ntensors, 
   int rc = check_tensors(tensors, ntensors, &total);
   if (!rc) rc = check_written(tensors, ntensors, outs);
   if (rc) return rc;
+  for (uint32_t i = 0; i < ntensors; ++i) {  // the norm is read while tensors are written
+    const u64 bytes = tensors[i].count * elem_bytes(tensors[i].type);
+    if (overlap(d_norm, 4, tensors[i].data, bytes) || (outs && overlap(d_norm, 4, outs[i], bytes))) return SVBGPU_EINVAL;
+  }
   if (!norm_given && (!ws || ((uintptr_t)ws & 255u) || ws_bytes < svbgpu_grad_workspace_bytes(ntensors))) return SVBGPU_EWORKSPACE;
   if (!host::device_ok()) return SVBGPU_ENODEVICE;
   if (norm_given) return launch_scale(tensors, ntensors, total, outs, d_norm, max_norm, S(stream));
@@ -274,6 +278,7 @@ int svbgpu_quantize_feedback_encode(int variant, int type, const void* d_grad, u
   if (overlap(d_grad, grad_bytes, d_residual_out, res_bytes) || overlap(d_out, out_bytes, d_grad, grad_bytes) ||
       overlap(d_out, out_bytes, d_residual, res_bytes) || overlap(d_out, out_bytes, d_residual_out, res_bytes))
     return SVBGPU_EINVAL;
+  if (d_norm && (overlap(d_norm, 4, d_residual_out, res_bytes) || overlap(d_norm, 4, d_out, out_bytes))) return SVBGPU_EINVAL;
   if (!host::device_ok()) return SVBGPU_ENODEVICE;
   hipStream_t st = S(stream);
   unsigned tag2 = 0;

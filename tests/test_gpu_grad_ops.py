@@ -55,6 +55,13 @@ SETS = {
     "table_edges": ([5 + i % 11 for i in range(160)], ["f32", "bf16"]),
     "over_one_table": ([3 + i % 17 for i in range(161)], ["bf16", "f32", "f16"]),
     "over_two_tables": ([1 + (i * 37) % 301 for i in range(481)], ["f16", "f32", "bf16"]),
+    # the set that one workgroup still takes, and the first that it does not
+    "small_by_bytes": ([CHUNK], ["f32"]),
+    "beyond_small_by_bytes": ([CHUNK + 1], ["f32"]),
+    "small_by_tensors": ([1 + 16 * i for i in range(64)], ["f32", "f16"]),
+    "beyond_small_by_tensors": ([1 + 16 * i for i in range(65)], ["f32", "f16"]),
+    "beyond_small_by_chunks": ([1025] * 33, ["f32"]),
+    "small_chunk_edges": ([1023, 1024, 1025, 2047, 2048, 2049, 4097], ["f32", "bf16"]),
     "with_holes": ([0 if i % 5 == 0 else i for i in range(300)], ["f32"]),
     "weights": ([1 << 20, 1024, 300007, 1, 65537], ["bf16", "f32"]),
 }
@@ -287,6 +294,46 @@ def test_feedback_encode(torch, codec, oracle, dtype, variant):
         assert np.array_equal(out[:want.size].cpu().numpy(), want)
 
 
+@pytest.mark.parametrize("n,dtype,variant", [
+    ((1 << 19) - 1, "f32", V0124), (1 << 19, "f16", V1234), ((1 << 21) - 1, "bf16", V0124), ((1 << 21) + 3, "f32", V1234),
+    (7 << 19, "f16", V0124), ((1 << 22) + 2, "bf16", V1234), ((1 << 23) - 3, "f32", V0124), ((1 << 23) + 1, "f32", V1234),
+    ((1 << 24) - 1, "bf16", V0124), ((1 << 24) + 5, "f32", V0124), ((1 << 24) + 30719, "bf16", V1234)])
+def test_feedback_of_every_tile_shape(torch, oracle, n, dtype, variant):
+    """The tile, the waves a tile and the cache policy change with the size: whole streams on both sides of each change,
+    gradients from far below a step to thousands of steps."""
+    import streamvbyte_amd as svb
+    codec = svb.DeviceCodec(n, "cuda:0")
+    g, r = gradients(torch, n, dtype, seed=n % 1000, far=3000.0)
+    norm = torch.tensor([1.25], device="cuda")
+    want, left = expected(oracle, variant, g, r, factor(1.25, 1.0), 64.0)
+    out = torch.full(((n + 3) // 4 + 4 * n + 16,), 0xA5, dtype=torch.uint8, device="cuda")
+    for _ in range(2):  # the second call finds the first one's words in the workspace
+        d_r = r.cuda()
+        _, size, _ = codec.quantize_feedback_encode(g.cuda(), 64.0, d_r, norm=norm, max_norm=1.0, out=out, variant=variant)
+        codec.check()
+        assert int(size.item()) == want.size
+        assert torch.equal(out[:want.size], torch.from_numpy(want).cuda())
+        assert bool((out[want.size:] == 0xA5).all())
+        assert same_bits(d_r, torch.from_numpy(left))
+
+
+@pytest.mark.parametrize("variant", [V0124, V1234])
+def test_feedback_of_incompressible_gradients(torch, codec, oracle, variant):
+    """Every width of integer up to four bytes in every group, beyond 2^22 too: the worst case of a tile's bytes."""
+    n = 150001
+    rng = np.random.default_rng(5)
+    x = (rng.standard_normal(n) * 2.0 ** rng.integers(0, 31, n)).astype(np.float32)
+    g, r = torch.from_numpy(x), torch.zeros(n)
+    want, left = expected(oracle, variant, g, r, np.float32(1.0), 1.0)
+    out, size, new = codec.quantize_feedback_encode(g.cuda(), 1.0, r.cuda(), variant=variant)
+    assert int(size.item()) == want.size and np.array_equal(out[:want.size].cpu().numpy(), want)
+    assert same_bits(new, torch.from_numpy(left))
+    big = torch.full((n,), -1.5e9)  # four bytes each
+    want, left = expected(oracle, variant, big, r, np.float32(1.0), 1.0)
+    out, size, new = codec.quantize_feedback_encode(big.cuda(), 1.0, r.cuda(), variant=variant)
+    assert int(size.item()) == want.size == (n + 3) // 4 + 4 * n and np.array_equal(out[:want.size].cpu().numpy(), want)
+
+
 def test_feedback_of_extremes(torch, codec, oracle):
     """Saturation at both ends of int32, infinities and NaN in gradient, residual and factor: such an element sends 0
     and keeps its residual; its neighbours do not notice."""
@@ -442,6 +489,33 @@ def test_captured_and_replayed(torch, oracle):
                                                               residual_out=torch.empty_like(residual))
         assert int(e_size.item()) == want.size and np.array_equal(e_out[:want.size].cpu().numpy(), want)
     codec.check()
+
+
+def test_a_graph_outlives_a_larger_eager_call(torch):
+    """A later call on more tensors takes a larger workspace; the captured one's stays what it is."""
+    import streamvbyte_amd as svb
+    codec = svb.DeviceCodec(1, "cuda:0")
+    small = make(torch, [200000, 300001], ["f32"], seed=90)
+    s, norm = svb.GradSet(small), torch.zeros(1, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        codec.grad_norm(s, out=norm)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            codec.grad_norm(s, out=norm)
+    torch.cuda.current_stream().wait_stream(side)
+    want = norm64(small, 2)
+    many = [torch.ones(3, device="cuda") for _ in range(9000)]
+    assert close_norm(codec.grad_norm(many), math.sqrt(27000))
+    bystanders = [torch.zeros(1 << 13, device="cuda") for _ in range(64)]  # what a freed workspace would be given to
+    for _ in range(3):
+        norm.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert close_norm(norm, want)
+        assert close_norm(codec.grad_norm(many), math.sqrt(27000))
+    assert not any(bool(b.any()) for b in bystanders)
 
 
 def test_on_streams_of_their_own(torch):

@@ -91,6 +91,18 @@ def test_clip_outputs():
     assert clip([(A, 10, F32), (None, 0, F32)], outs=[B, None]) == ENODEVICE
 
 
+def test_the_norm_lies_apart():
+    """It is read while tensors are written."""
+    rows = [(A, 10, F32), (B, 3, BF16)]
+    for d_norm in (A, A + 36, B, B + 4):
+        assert clip(rows, d_norm=d_norm) == EINVAL, hex(d_norm)
+        assert clip(rows, outs=[0x30_0000, 0x31_0000], d_norm=d_norm) == EINVAL
+        assert norm(rows, d_norm=d_norm) == ENODEVICE               # written when everything is read
+    assert clip(rows, d_norm=A + 40) == ENODEVICE and clip(rows, d_norm=B + 8) == ENODEVICE
+    assert clip(rows, outs=[0x30_0000, 0x31_0000], d_norm=0x30_0000 + 36) == EINVAL
+    assert clip(rows, outs=[0x30_0000, 0x31_0000], d_norm=0x31_0004, given=1) == EINVAL
+
+
 def test_feedback_arguments():
     lib = svb.load()
     n = 1000
@@ -118,10 +130,12 @@ def test_feedback_arguments():
     assert call(out=A + 4 * n - 1) == EINVAL and call(out=A + 4 * n) == ENODEVICE
     assert call(out=B - room + 1) == EINVAL and call(out=B - room) == ENODEVICE
     assert call(r_out=0x30_0000, out=0x30_0000 + 4 * n - 1) == EINVAL
+    assert call(norm=B) == EINVAL and call(norm=B + 4 * n - 4) == EINVAL and call(norm=B + 4 * n) == ENODEVICE
+    assert call(norm=0x40_0000) == EINVAL and call(norm=A) == ENODEVICE                # a gradient may hold it
 
 
 def test_sets_look_their_tensors_over():
-    with pytest.raises(ValueError, match="not on a device"):
+    with pytest.raises(ValueError, match="not a dense tensor on a device"):
         svb.GradSet([torch.zeros(3)])
     assert len(svb.GradSet([])) == 0
     with pytest.raises(ValueError, match="0 tensors, but 1 outputs"):

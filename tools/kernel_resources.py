@@ -1,10 +1,17 @@
 #!/usr/bin/env python3
-"""Print one line per kernel: VGPRs, SGPRs, scratch, LDS, occupancy (hipcc remarks)."""
+"""Print one line per kernel: VGPRs, SGPRs, scratch, LDS, occupancy (hipcc remarks).
+
+    python tools/kernel_resources.py [--unit svb_grad] [hipcc flags]
+"""
 import os, re, subprocess, sys
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + sys.argv[1:] + [ "-I", os.path.join(ROOT, "include"),
+args = sys.argv[1:]
+unit = "svb_api"
+if args[:1] == ["--unit"]:
+    unit, args = args[1], args[2:]
+cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + args + [ "-I", os.path.join(ROOT, "include"),
        "--cuda-device-only", "-c", "-Rpass-analysis=kernel-resource-usage", "-o", "/dev/null",
-       os.path.join(ROOT, "streamvbyte_amd/csrc/svb_api.hip")]
+       os.path.join(ROOT, f"streamvbyte_amd/csrc/{unit}.hip")]
 out = subprocess.run(cmd, capture_output=True, text=True).stderr
 cur = {}
 rows = []
