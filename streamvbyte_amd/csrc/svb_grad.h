@@ -494,29 +494,35 @@ __device__ __forceinline__ u32 present_lane(u64 wt_first, int lane, u32 count) {
 }
 constexpr u32 kFeedMaxWaves = 15;  // data waves of a workgroup, at most
 // One pass.  A workgroup takes tiles off a ticket, QW wave tiles (of 1024 values) for each of its first nw waves; its
-// last wave, the scan wave, draws the tickets and finds the tiles' places by look-back.  A data wave's round:
-//     quantise (values and residuals have arrived), send the new residuals off, count the bytes | barrier A |
-//     assemble the bytes in LDS, request the next tile's values and residuals                  | barrier B | copy out
+// last wave, the scan wave, draws the tickets and finds the tiles' places by look-back.  A data wave's round k:
+//     quantise (values and residuals have arrived), send the new residuals off, count the bytes   | barrier A |
+//     assemble the bytes in LDS, request the next tile's values and residuals
+//     DEFER: copy out the tile of round k - 1, whose bytes have waited in the other image;  else: | barrier B | copy out
 // and the scan wave's:
-//     draw the next ticket | A | publish the tile's bytes, look back until the place is known | B |
-// so a tile's look-back runs beside its assembly and the next tile's loads, and the polls never stand in a queue with
-// a data wave's loads and stores.  The barriers order LDS only: __syncthreads would wait for the stores as well.
-// Between a tile's ticket and its publication a workgroup waits only for tiles with smaller tickets: the chain ends.
+//     draw the next ticket (DEFER: after the publication) | A | publish the tile's bytes, look back until the place is known | B
+// (without B in all but the last round of DEFER),
+// so a tile's look-back runs beside its assembly and the next tile's loads (DEFER: beside a whole round), and the polls
+// never stand in a queue with a data wave's loads and stores.  The loads go out only when the bytes are assembled: sent
+// at the start of the round they are ahead of the polls in the CU's memory queue, which lengthens every look-back by
+// more than they gain (2^25 values 107 us instead of 87).  The barriers order LDS only: __syncthreads would wait for the
+// stores as well.  What the scan wave hands over has two places, the byte counts three: nobody who still reads round k
+// is passed by a writer of the round that takes the same place.  Between a tile's ticket and its publication a workgroup
+// waits only for tiles with smaller tickets: the chain ends.
 //
-// Bound by memory, 12.8 B a value for float32 (0124): 2^26 values in 150 us = 5.7 TB/s; without look-back and tickets
-// (wrong places) the same kernel takes 135 us, and with nothing but the elementwise part 134.  What it took to get
-// there from 187 us, the tile-at-a-time form of k_encode: assembling before the place is known (165), half the
-// instructions a value (feed_group, the one-byte quarters of assemble), one workgroup of 15 data waves per CU instead of
-// two (158; a look-back's answers come slower the more tiles wait) and 30 wave tiles a tile instead of 15 (150).
-template <int V, int T, int QW, int NT>
-__global__ __launch_bounds__(kFeedMaxWaves * 64 + 64, 4) void k_feedback_encode(const u8* __restrict__ grad, u32 count, u32 n_tiles, u32 nw,
-                                                                             u8* __restrict__ out, FeedArgs fa,
-                                                                             WsHeader* __restrict__ hdr, LbWords lb,
-                                                                             u64* __restrict__ written) {
-  __shared__ EncWaveLds s_lds[kFeedMaxWaves * QW];
-  __shared__ u32 s_wave_tot[2][kFeedMaxWaves];
-  __shared__ u64 s_prefix;
-  __shared__ u32 s_first, s_next;
+// Bound by memory, 12.8 B a value for float32 (0124): 2^26 values in 147 us = 5.9 TB/s; nothing but the elementwise part
+// takes 134.  What it took to get there from 187 us, the tile-at-a-time form of k_encode: assembling before the place is
+// known (165), half the instructions a value (feed_group, the one-byte quarters of assemble), one workgroup of 15 data
+// waves per CU instead of two (158; a look-back takes the longer the more tiles are in flight, about 20 ns each), 30 wave
+// tiles a tile (151) or, instead, the deferred copy (147).
+template <int V, int T, int QW, bool DEFER, int NT>
+__global__ __launch_bounds__(kFeedMaxWaves * 64 + 64, 4) void k_feedback_encode(const u8* __restrict__ grad, u32 count, u32 n_tiles,
+                                                                                u32 nw, u8* __restrict__ out, FeedArgs fa,
+                                                                                WsHeader* __restrict__ hdr, LbWords lb,
+                                                                                u64* __restrict__ written) {
+  __shared__ EncWaveLds s_lds[DEFER ? 2 : 1][kFeedMaxWaves * QW];
+  __shared__ u32 s_wave_tot[3][kFeedMaxWaves];
+  __shared__ u64 s_prefix[2];
+  __shared__ u32 s_first, s_next[2];
   const int lane = lane_id(), wave = wave_id();
   const u64 keylen = ((u64)count + 3) >> 2;
   if (wave == (int)nw) {  // the scan wave
@@ -530,21 +536,28 @@ __global__ __launch_bounds__(kFeedMaxWaves * 64 + 64, 4) void k_feedback_encode(
     if (lane == 0) s_first = tile;
     lds_barrier();
     if (tile >= n_tiles) return;
-    for (int buf = 0;; buf ^= 1) {
-      const u32 next = once ? n_tiles : draw();
-      if (lane == 0) s_next = next;
+    u32 next = n_tiles;
+    for (u32 k = 0;; ++k) {
+      if (!DEFER || k == 0) {
+        next = once ? n_tiles : draw();
+        if (lane == 0) s_next[k & 1] = next;
+      }
       lds_barrier();  // A
-      const u32 tot = lane < (int)nw ? s_wave_tot[buf][lane] : 0u;
-      const u32 tile_tot = wave_sum(tot);
-      const u64 excl = lb2_exclusive_prefix<2>(lb, tile, tile_tot, lane, &hdr->error);
+      const u32 tile_tot = wave_sum(lane < (int)nw ? s_wave_tot[k % 3][lane] : 0u);
+      lb2_publish(lb, tile, tile_tot, lane, &hdr->error);
+      u32 after = n_tiles;
+      if (DEFER && next < n_tiles) after = draw();
+      const u64 excl = lb2_resolve<2>(lb, tile, tile_tot, lane, &hdr->error);
       if (lane == 0) {
-        s_prefix = excl;
+        s_prefix[k & 1] = excl;
+        if (DEFER) s_next[(k + 1) & 1] = after;
         if (tile == n_tiles - 1 && written) *written = keylen + excl + tile_tot;
         if (tile == 0u) reset_other_ticket(hdr);
       }
-      lds_barrier();  // B
+      if (!DEFER || next >= n_tiles) lds_barrier();  // B
       if (next >= n_tiles) return;
       tile = next;
+      next = after;
     }
   }
   const float c = fa.norm ? clip_factor(*fa.norm, fa.limit) : 1.0f;
@@ -569,12 +582,26 @@ __global__ __launch_bounds__(kFeedMaxWaves * 64 + 64, 4) void k_feedback_encode(
       }
     }
   };
+  u32 done = 0;          // the tile of round `k` that `totals` is about
+  u32 totals[QW] = {};   // bytes of its wave tiles
+  auto finish = [&](u32 k) {
+    u64 doff = keylen + s_prefix[k & 1];
+    for (int w = 0; w < wave; ++w) doff += s_wave_tot[k % 3][w];
+#pragma unroll
+    for (int q = 0; q < QW; ++q) {
+      const u64 wt_first = first_of(done, q);
+      if (wt_first < count)
+        copy_out<(NT & kNtStores) != 0>(s_lds[DEFER ? k & 1 : 0][wave * QW + q], totals[q],
+                                        (u32)((min((u64)kWtInts, (u64)count - wt_first) + 3) >> 2), lane, out + doff, out + (wt_first >> 2));
+      doff += totals[q];
+    }
+  };
   lds_barrier();
   u32 tile = __builtin_amdgcn_readfirstlane(s_first);
   if (tile >= n_tiles) return;
 #pragma unroll
   for (int q = 0; q < QW; ++q) request(tile, q);
-  for (int buf = 0;; buf ^= 1) {
+  for (u32 k = 0;; ++k) {
     uint4 x[QW][4];  // the zigzagged integers
     u32 k4[QW];      // their groups' keys
     u32 lane_tot = 0;
@@ -595,8 +622,8 @@ __global__ __launch_bounds__(kFeedMaxWaves * 64 + 64, 4) void k_feedback_encode(
         } else {
           const u32 nv = present(first, count);
 #pragma unroll
-          for (u32 k = 0; k < 4; ++k)
-            if (k < nv) fa.r_out[first + k] = rv[k];
+          for (u32 i = 0; i < 4; ++i)
+            if (i < nv) fa.r_out[first + i] = rv[i];
           zero_absent(x[q][j], first, count);
           key &= (1u << (2u * nv)) - 1u;
         }
@@ -607,10 +634,10 @@ __global__ __launch_bounds__(kFeedMaxWaves * 64 + 64, 4) void k_feedback_encode(
       lane_tot += full || V == V0124 ? word_len<V>(keys, 16u) : word_len<V>(keys, present_lane(wt_first, lane, count));
     }
     const u32 wave_tot = wave_sum(lane_tot);
-    if (lane == 0) s_wave_tot[buf][wave] = wave_tot;
+    if (lane == 0) s_wave_tot[k % 3][wave] = wave_tot;
     lds_barrier();  // A
-    const u32 next = __builtin_amdgcn_readfirstlane(s_next);
-    u32 totals[QW];
+    const u32 next = __builtin_amdgcn_readfirstlane(s_next[k & 1]);
+    u32 mine[QW];
 #pragma unroll
     for (int q = 0; q < QW; ++q) {
       const u64 wt_first = first_of(tile, q);
@@ -625,23 +652,21 @@ __global__ __launch_bounds__(kFeedMaxWaves * 64 + 64, 4) void k_feedback_encode(
 #pragma unroll
       for (int j = 0; j < 4; ++j) g[j] = ((k4[q] >> (8 * j)) & 0xFFu) | (((lens4 >> (8 * j)) & 0xFFu) << 24);
       const WavePlaces places = wave_places(g, lane);
-      totals[q] = places.total;
-      if (full) assemble<V, true>(x[q], g, places, lane, s_lds[wave * QW + q]);
-      else assemble<V, false>(x[q], g, places, lane, s_lds[wave * QW + q]);
+      mine[q] = places.total;
+      EncWaveLds& S = s_lds[DEFER ? k & 1 : 0][wave * QW + q];
+      if (full) assemble<V, true>(x[q], g, places, lane, S);
+      else assemble<V, false>(x[q], g, places, lane, S);
       __builtin_amdgcn_sched_barrier(0);
       request(next, q);
       __builtin_amdgcn_sched_barrier(0);
     }
-    lds_barrier();  // B
-    u64 doff = keylen + s_prefix;
-    for (int w = 0; w < wave; ++w) doff += s_wave_tot[buf][w];
+    if (DEFER && k) finish(k - 1);
+    done = tile;
 #pragma unroll
-    for (int q = 0; q < QW; ++q) {
-      const u64 wt_first = first_of(tile, q);
-      if (wt_first < count)
-        copy_out<(NT & kNtStores) != 0>(s_lds[wave * QW + q], totals[q], (u32)((min((u64)kWtInts, (u64)count - wt_first) + 3) >> 2), lane,
-                                        out + doff, out + (wt_first >> 2));
-      doff += totals[q];
+    for (int q = 0; q < QW; ++q) totals[q] = mine[q];
+    if (!DEFER || next >= n_tiles) {
+      lds_barrier();  // B
+      finish(k);
     }
     if (next >= n_tiles) return;
     tile = next;

@@ -200,7 +200,7 @@ int run(int kind, const svbgpu_tensor* t, uint32_t n, u64 total, void* const* ou
   return run_kind<kNormEuclid>(t, n, total, outs, clip, limit, d_norm, ws, st);
 }
 
-template <int V, int T, int QW, int NT>
+template <int V, int T, int QW, bool DEFER, int NT>
 void launch_feedback(u32 nw, const void* grad, uint32_t count, uint8_t* d_out, const FeedArgs& fa, void* ws, unsigned tag2,
                      uint64_t* d_written, hipStream_t st) {
   const WsLayout L = ws_layout(count);  // has a look-back word per kWaves wave tiles: nw * QW >= kWaves
@@ -208,26 +208,30 @@ void launch_feedback(u32 nw, const void* grad, uint32_t count, uint8_t* d_out, c
   const u32 grid = std::min<u32>(tiles, (u32)std::max(host::device_cus(), 1));
   WsHeader* h = reinterpret_cast<WsHeader*>(static_cast<char*>(ws) + ((tag2 >> 3) & 1u) * 8);
   const LbWords lb{reinterpret_cast<u64*>(static_cast<char*>(ws) + L.off_status), (u32)((L.off_lb_group - L.off_status) / 8), tag2};
-  hipLaunchKernelGGL((k_feedback_encode<V, T, QW, NT>), dim3(grid), dim3((nw + 1) * 64), 0, st, static_cast<const u8*>(grad), count,
+  hipLaunchKernelGGL((k_feedback_encode<V, T, QW, DEFER, NT>), dim3(grid), dim3((nw + 1) * 64), 0, st, static_cast<const u8*>(grad), count,
                      tiles, nw, d_out, fa, h, lb, d_written);
 }
 // The tile by size.  A large tile means few look-backs, a small one that a short stream reaches more of the device and
-// that the last round of workgroups is fuller.  Measured with float32, 0124, us for QW x nw wave tiles a tile:
+// that the last round of workgroups is fuller; the deferred copy hides the look-backs of many rounds.  Measured with
+// float32, 0124, us for QW x nw wave tiles a tile:
 //     2^18 values: 1x4 6.3, 1x8 6.7, 1x15 7.9                2^20: 1x4 10.4, 1x8 8.6, 1x15 9.0, 2x15 12.7
-//     3 * 2^20: 1x8 17.5, 1x15 13.4, 2x15 14.9               2^22: 1x15 17.4, 2x15 16.5
-//     6 * 2^20: 1x15 23.6, 2x15 19.8                         2^24: 1x15 49.3, 2x11 48.0, 2x15 50.9
-//     2^25: 1x15 86.7, 2x11 82.7, 2x15 83.9
-// Non-temporal stores from 2^23 values up and loads from 2^24, where what a call touches no longer stays in the Infinity
-// Cache (2^23: 30 us, with such stores 26, with the loads too 30; 2^26: 161, 156, 151).
+//     2^21: 1x8 12.4, 1x15 11.5, 2x12 12.7                   3 * 2^20: 1x8 17.5, 1x15 13.4, 2x12 14.3
+//     2^22: 1x15 17.8, 2x12 15.6                             6 * 2^20: 1x15 22.5, 2x12 20.2
+//     2^23: 1x15 27.1, 2x12 27.4, deferred 29.0              12 * 2^20: 1x15 40.7, 2x12 38.3, deferred 40.1
+//     2^24: 1x15 49.7, 2x12 48.4, deferred 47.7              2^25: 1x15 86.9, 2x12 83.3, deferred 80.3
+//     2^26: 1x15 162.6, 2x15 152.1, deferred 146.3
+// Non-temporal stores where what a call touches begins to fill the Infinity Cache, non-temporal loads where it is far
+// beyond it (2^22, 2x12: 16.1 us, with such stores 15.6, with the loads too 18.3; 2^24: 53.8, 49.8, 48.4).
 template <int V, int T>
 void launch_feedback(const void* grad, uint32_t count, uint8_t* d_out, const FeedArgs& fa, void* ws, unsigned tag2, uint64_t* d_written,
                      hipStream_t st) {
   const u32 m = count >> 19;  // in half millions
-  if (m < 4) launch_feedback<V, T, 1, 0>(m < 1 ? 4 : 8, grad, count, d_out, fa, ws, tag2, d_written, st);
-  else if (m < 7) launch_feedback<V, T, 1, 0>(15, grad, count, d_out, fa, ws, tag2, d_written, st);
-  else if (m < 16) launch_feedback<V, T, 2, 0>(15, grad, count, d_out, fa, ws, tag2, d_written, st);
-  else if (m < 32) launch_feedback<V, T, 1, kNtStores>(15, grad, count, d_out, fa, ws, tag2, d_written, st);
-  else launch_feedback<V, T, 2, kNtLoads | kNtStores>(11, grad, count, d_out, fa, ws, tag2, d_written, st);
+  if (m < 3) launch_feedback<V, T, 1, false, 0>(m < 1 ? 4 : 8, grad, count, d_out, fa, ws, tag2, d_written, st);
+  else if (m < 7) launch_feedback<V, T, 1, false, 0>(15, grad, count, d_out, fa, ws, tag2, d_written, st);
+  else if (m < 16) launch_feedback<V, T, 2, false, kNtStores>(12, grad, count, d_out, fa, ws, tag2, d_written, st);
+  else if (m < 24) launch_feedback<V, T, 1, false, kNtStores>(15, grad, count, d_out, fa, ws, tag2, d_written, st);
+  else if (m < 32) launch_feedback<V, T, 2, false, kNtStores>(12, grad, count, d_out, fa, ws, tag2, d_written, st);
+  else launch_feedback<V, T, 1, true, kNtLoads | kNtStores>(15, grad, count, d_out, fa, ws, tag2, d_written, st);
 }
 
 }  // namespace
