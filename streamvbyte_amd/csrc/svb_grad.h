@@ -509,11 +509,12 @@ constexpr u32 kFeedMaxWaves = 15;  // data waves of a workgroup, at most
 // is passed by a writer of the round that takes the same place.  Between a tile's ticket and its publication a workgroup
 // waits only for tiles with smaller tickets: the chain ends.
 //
-// Bound by memory, 12.8 B a value for float32 (0124): 2^26 values in 147 us = 5.9 TB/s; nothing but the elementwise part
+// Bound by memory, 12.8 B a value for float32 (0124): 2^26 values in 140 us = 6.2 TB/s; nothing but the elementwise part
 // takes 134.  What it took to get there from 187 us, the tile-at-a-time form of k_encode: assembling before the place is
 // known (165), half the instructions a value (feed_group, the one-byte quarters of assemble), one workgroup of 15 data
-// waves per CU instead of two (158; a look-back takes the longer the more tiles are in flight, about 20 ns each), 30 wave
-// tiles a tile (151) or, instead, the deferred copy (147).
+// waves per CU instead of two (158; a look-back takes the longer the more tiles are in flight, about 20 ns each), the
+// deferred copy (144; 30 wave tiles a tile without it 151), 256 tile words a look-back instead of 128 (140: all that are
+// in flight, so none waits for a group's leader).  The ticket drawn after the look-back instead of before it costs 10 us.
 template <int V, int T, int QW, bool DEFER, int NT>
 __global__ __launch_bounds__(kFeedMaxWaves * 64 + 64, 4) void k_feedback_encode(const u8* __restrict__ grad, u32 count, u32 n_tiles,
                                                                                 u32 nw, u8* __restrict__ out, FeedArgs fa,
@@ -547,7 +548,7 @@ __global__ __launch_bounds__(kFeedMaxWaves * 64 + 64, 4) void k_feedback_encode(
       lb2_publish(lb, tile, tile_tot, lane, &hdr->error);
       u32 after = n_tiles;
       if (DEFER && next < n_tiles) after = draw();
-      const u64 excl = lb2_resolve<2>(lb, tile, tile_tot, lane, &hdr->error);
+      const u64 excl = lb2_resolve<4>(lb, tile, tile_tot, lane, &hdr->error);
       if (lane == 0) {
         s_prefix[k & 1] = excl;
         if (DEFER) s_next[(k + 1) & 1] = after;

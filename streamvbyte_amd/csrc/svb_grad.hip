@@ -211,26 +211,26 @@ void launch_feedback(u32 nw, const void* grad, uint32_t count, uint8_t* d_out, c
   hipLaunchKernelGGL((k_feedback_encode<V, T, QW, DEFER, NT>), dim3(grid), dim3((nw + 1) * 64), 0, st, static_cast<const u8*>(grad), count,
                      tiles, nw, d_out, fa, h, lb, d_written);
 }
-// The tile by size.  A large tile means few look-backs, a small one that a short stream reaches more of the device and
-// that the last round of workgroups is fuller; the deferred copy hides the look-backs of many rounds.  Measured with
-// float32, 0124, us for QW x nw wave tiles a tile:
-//     2^18 values: 1x4 6.3, 1x8 6.7, 1x15 7.9                2^20: 1x4 10.4, 1x8 8.6, 1x15 9.0, 2x15 12.7
-//     2^21: 1x8 12.4, 1x15 11.5, 2x12 12.7                   3 * 2^20: 1x8 17.5, 1x15 13.4, 2x12 14.3
-//     2^22: 1x15 17.8, 2x12 15.6                             6 * 2^20: 1x15 22.5, 2x12 20.2
-//     2^23: 1x15 27.1, 2x12 27.4, deferred 29.0              12 * 2^20: 1x15 40.7, 2x12 38.3, deferred 40.1
-//     2^24: 1x15 49.7, 2x12 48.4, deferred 47.7              2^25: 1x15 86.9, 2x12 83.3, deferred 80.3
-//     2^26: 1x15 162.6, 2x15 152.1, deferred 146.3
+// The tile by size.  A large tile means few look-backs, a small one that a short stream reaches more of the device; the
+// deferred copy hides the look-backs where a workgroup takes several tiles.  Measured with float32, 0124, us for QW x nw
+// wave tiles a tile:
+//     2^18 values: 1x4 6.3, 1x8 6.7, 1x15 7.9                2^20: 1x4 10.4, 1x8 8.6, 1x15 8.9
+//     2^21: 1x8 12.4, 1x15 11.3, 2x12 12.2                   3 * 2^20: 1x15 13.2, 2x12 13.8, deferred 13.6
+//     2^22: 1x15 17.4, 2x12 15.6, deferred 17.1              6 * 2^20: 1x15 22.3, 2x12 20.0, deferred 20.6
+//     7 * 2^20: 2x12 26.4, 2x15 22.1, deferred 23.6          2^23: 1x15 27.0, 2x12 27.2, deferred 25.3
+//     12 * 2^20: 1x15 40.6, 2x12 37.3, deferred 35.6         2^24: 1x15 51.2, 2x12 48.7, deferred 45.0
+//     2^26: 1x15 163, 2x15 152, deferred 140
+// Two wave tiles a wave are for streams that are one round of the device's 256 CUs that way and more with one.
 // Non-temporal stores where what a call touches begins to fill the Infinity Cache, non-temporal loads where it is far
-// beyond it (2^22, 2x12: 16.1 us, with such stores 15.6, with the loads too 18.3; 2^24: 53.8, 49.8, 48.4).
+// beyond it (deferred: 2^23 27.9 us, with such stores 25.3, with the loads too 27.4; 2^24 47.5, 45.0, 44.2).
 template <int V, int T>
 void launch_feedback(const void* grad, uint32_t count, uint8_t* d_out, const FeedArgs& fa, void* ws, unsigned tag2, uint64_t* d_written,
                      hipStream_t st) {
   const u32 m = count >> 19;  // in half millions
   if (m < 3) launch_feedback<V, T, 1, false, 0>(m < 1 ? 4 : 8, grad, count, d_out, fa, ws, tag2, d_written, st);
   else if (m < 7) launch_feedback<V, T, 1, false, 0>(15, grad, count, d_out, fa, ws, tag2, d_written, st);
-  else if (m < 16) launch_feedback<V, T, 2, false, kNtStores>(12, grad, count, d_out, fa, ws, tag2, d_written, st);
-  else if (m < 24) launch_feedback<V, T, 1, false, kNtStores>(15, grad, count, d_out, fa, ws, tag2, d_written, st);
-  else if (m < 32) launch_feedback<V, T, 2, false, kNtStores>(12, grad, count, d_out, fa, ws, tag2, d_written, st);
+  else if (m < 15) launch_feedback<V, T, 2, false, kNtStores>(m < 12 ? 12 : 15, grad, count, d_out, fa, ws, tag2, d_written, st);
+  else if (m < 32) launch_feedback<V, T, 1, true, kNtStores>(15, grad, count, d_out, fa, ws, tag2, d_written, st);
   else launch_feedback<V, T, 1, true, kNtLoads | kNtStores>(15, grad, count, d_out, fa, ws, tag2, d_written, st);
 }
 

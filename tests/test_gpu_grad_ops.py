@@ -295,8 +295,9 @@ def test_feedback_encode(torch, codec, oracle, dtype, variant):
 
 
 @pytest.mark.parametrize("n,dtype,variant", [
-    ((1 << 19) - 1, "f32", V0124), (1 << 19, "f16", V1234), ((1 << 21) - 1, "bf16", V0124), ((1 << 21) + 3, "f32", V1234),
-    (7 << 19, "f16", V0124), ((1 << 22) + 2, "bf16", V1234), ((1 << 23) - 3, "f32", V0124), ((1 << 23) + 1, "f32", V1234),
+    ((1 << 19) - 1, "f32", V0124), (1 << 19, "f16", V1234), ((3 << 19) - 1, "bf16", V0124), ((3 << 19) + 3, "f32", V1234),
+    ((7 << 19) - 1, "f32", V0124), (7 << 19, "f16", V0124), ((6 << 20) - 2, "bf16", V1234), ((6 << 20) + 1, "f32", V0124),
+    ((15 << 19) - 3, "f32", V0124), ((15 << 19) + 1, "f32", V1234), ((15 << 19) + 2, "f16", V0124),
     ((1 << 24) - 1, "bf16", V0124), ((1 << 24) + 5, "f32", V0124), ((1 << 24) + 30719, "bf16", V1234)])
 def test_feedback_of_every_tile_shape(torch, oracle, n, dtype, variant):
     """The tile, the waves a tile and the cache policy change with the size: whole streams on both sides of each change,
