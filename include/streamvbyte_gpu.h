@@ -163,7 +163,7 @@ size_t svbgpu_workspace_bytes(uint32_t count);
 
 /* Optional, once per workspace (no counterpart in the reference, which needs no scratch): zeroes the
  * workspace on `stream` and remembers its address.  Calls that chain tiles through look-back words
- * (svbgpu_encode, svbgpu_quantize_encode, svbgpu_encode64, svbgpu_zigzag_delta_decode) and
+ * (svbgpu_encode, svbgpu_quantize_encode, svbgpu_quantize_feedback_encode, svbgpu_encode64, svbgpu_zigzag_delta_decode) and
  * svbgpu_validate then skip the clearing launch they otherwise start with (4-5 us a call, 5 % of an
  * encode of 2^26 values): every such call marks the words it writes with a tag of its own, so what
  * earlier calls left behind reads as empty.  Rules: the workspace must not be written by anything

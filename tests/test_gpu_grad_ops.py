@@ -189,6 +189,60 @@ def test_clip_with_a_norm_that_is_given(torch, codec):
             assert same_bits(g, clipped(s, factor(value, 1.0))), value
 
 
+def test_a_given_norm_and_outputs(torch, codec):
+    """The two together, on a set larger and one smaller than one workgroup takes."""
+    import streamvbyte_amd as svb
+    for sizes in ([700, 3], [90001, 17, 4096], [2, 5] * 100):
+        src = make(torch, sizes, ["bf16", "f32", "f16"], seed=len(sizes))
+        keep = [t.clone() for t in src]
+        outs = [torch.full_like(t, 9.0) for t in src]
+        given = torch.tensor(7.0, device="cuda")  # without a dimension
+        codec.clip_grads(svb.GradSet(src, out=outs), 2.0, norm=given)
+        for k, t, y in zip(keep, src, outs):
+            assert same_bits(t, k) and same_bits(y, clipped(k, factor(7.0, 2.0)))
+
+
+def test_what_the_methods_refuse(torch, codec):
+    import streamvbyte_amd as svb
+    x, h = torch.randn(100).cuda(), torch.randn(64, 64).cuda()
+    keep = x.clone()
+    for wrong in ([x, x], [x, x[10:20]], [h[:8], h[7:]]):
+        with pytest.raises(svb.SvbError, match="invalid argument"):
+            codec.clip_grads(wrong, 1e-3)
+    for wrong in ([h[:, 3]], [h[::2]], [x[:1].expand(9)], [x.double()], [x.int()], [x.cpu()], [torch.eye(4).to_sparse().cuda()]):
+        for call in (codec.grad_norm, lambda g: codec.clip_grads(g, 1.0)):
+            with pytest.raises(ValueError):
+                call(wrong)
+    for p in (0, 3, -1, "fro"):
+        with pytest.raises(ValueError):
+            codec.grad_norm([x], p)
+    for limit in (-1.0, math.nan):
+        with pytest.raises(ValueError):
+            codec.clip_grads([x], limit)
+    for out in ([h], [x, x], [x.half()], [torch.empty(50, 2, device="cuda")]):
+        with pytest.raises(ValueError):
+            svb.GradSet([x], out=out)
+    with pytest.raises(svb.SvbError):  # shifted against itself
+        codec.clip_grads(svb.GradSet([x[:50]], out=[x[1:51]]), 1e-3)
+    for norm in (torch.zeros(2, device="cuda"), torch.zeros(1), torch.zeros(1, device="cuda", dtype=torch.float64)):
+        with pytest.raises(ValueError):
+            codec.clip_grads([x], 1.0, norm=norm)
+        with pytest.raises(ValueError):
+            codec.grad_norm([x], out=norm)
+    r = torch.zeros(100, device="cuda")
+    for change in (dict(grad=x.double()), dict(grad=x[::2]), dict(residual=r[:50]), dict(residual=r.half()), dict(residual=r.cpu()),
+                   dict(out=torch.empty(10, dtype=torch.uint8, device="cuda")), dict(out=torch.empty(1000, device="cuda")),
+                   dict(residual_out=r[1:]), dict(norm=torch.zeros(2, device="cuda")), dict(grad=torch.zeros((1 << 21) + 1, device="cuda"))):
+        with pytest.raises(ValueError):
+            codec.quantize_feedback_encode(**dict(dict(grad=x, scale=64.0, residual=r), **change))
+    for change in (dict(scale=0.0), dict(scale=-1.0), dict(scale=INF), dict(variant=2), dict(residual=x), dict(norm=r[5:6], max_norm=1.0),
+                   dict(norm=torch.ones(1, device="cuda"), max_norm=-1.0)):
+        with pytest.raises(svb.SvbError):
+            codec.quantize_feedback_encode(**dict(dict(grad=x, scale=64.0, residual=r), **change))
+    torch.cuda.synchronize()
+    assert torch.equal(x, keep) and not bool(r.any())  # nothing ran
+
+
 def test_clip_of_what_is_not_finite(torch, codec):
     for bad in (INF, math.nan):
         src = make(torch, [100, 33000], ["f32", "f16"], seed=12)
@@ -490,6 +544,80 @@ def test_captured_and_replayed(torch, oracle):
                                                               residual_out=torch.empty_like(residual))
         assert int(e_size.item()) == want.size and np.array_equal(e_out[:want.size].cpu().numpy(), want)
     codec.check()
+
+
+def test_two_graphs_of_one_codec(torch, oracle):
+    """Both hold the codec's workspaces; replayed in turn on one stream, in any order, each gives what it gave."""
+    import streamvbyte_amd as svb
+    n = 50001
+    codec = svb.DeviceCodec(n, "cuda:0")
+    side = torch.cuda.Stream()
+    parts = []
+    for i in range(2):
+        g, r = gradients(torch, n - 20000 * i, "f32", seed=200 + i)
+        d = dict(g=g.cuda(), r=r.cuda(), new=torch.zeros_like(r).cuda(), norm=torch.zeros(1, device="cuda"), size=torch.zeros(1, dtype=torch.int64, device="cuda"))
+        d["out"] = torch.zeros(svb.streamvbyte_max_compressedbytes(g.numel()), dtype=torch.uint8, device="cuda")
+        d["set"] = svb.GradSet([d["g"]])
+        want, left = expected(oracle, V0124, g, r, factor(norm64([g], 2), 0.5), 64.0)
+        parts.append((d, want, left, norm64([g], 2)))
+    graphs = []
+    for d, *_ in parts:
+        def step():
+            codec.grad_norm(d["set"], out=d["norm"])
+            z = codec.quantize_feedback_encode(d["g"], 64.0, d["r"], norm=d["norm"], max_norm=0.5, out=d["out"], residual_out=d["new"])[1]
+            d["size"].copy_(z)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                step()
+        torch.cuda.current_stream().wait_stream(side)
+        graphs.append(graph)
+    for order in ((0, 1), (1, 0), (1, 1, 0, 0)):
+        for d, *_ in parts:
+            d["out"].zero_(), d["new"].zero_(), d["norm"].zero_(), d["size"].zero_()
+        for i in order:
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for d, want, left, n64 in parts:
+            assert close_norm(d["norm"], n64)
+            c = factor(d["norm"].item(), 0.5)
+            if c == factor(n64, 0.5):  # the float32 norm is the nearest one, so it nearly always is
+                assert int(d["size"].item()) == want.size and np.array_equal(d["out"][:want.size].cpu().numpy(), want)
+                assert same_bits(d["new"], torch.from_numpy(left))
+        assert float(codec.grad_norm([parts[0][0]["g"]])) == float(parts[0][0]["norm"])  # and eager calls in between
+    codec.check()
+
+
+def test_from_several_threads(torch, oracle):
+    """A codec, a stream and buffers a thread, all at once."""
+    import threading
+    import streamvbyte_amd as svb
+    n, failures = 120007, []
+    g, r = gradients(torch, n, "bf16", seed=300)
+    want, left = expected(oracle, V1234, g, r, factor(2.0, 1.0), 64.0)
+
+    def work():
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                codec = svb.DeviceCodec(n, "cuda:0")
+                d_g, norm = g.cuda(), torch.tensor([2.0], device="cuda")
+                for _ in range(10):
+                    out, size, new = codec.quantize_feedback_encode(d_g, 64.0, r.cuda(), norm=norm, max_norm=1.0, variant=V1234)
+                    ok = int(size.item()) == want.size and np.array_equal(out[:want.size].cpu().numpy(), want)
+                    ok = ok and same_bits(new, torch.from_numpy(left)) and close_norm(codec.grad_norm([d_g, d_g]), norm64([g, g], 2))
+                    if not ok:
+                        failures.append("wrong")
+        except Exception as e:  # noqa: BLE001 -- reported by the test
+            failures.append(repr(e))
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures[:3]
 
 
 def test_a_graph_outlives_a_larger_eager_call(torch):
