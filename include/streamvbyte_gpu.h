@@ -300,7 +300,8 @@ int svbgpu_grad_clip(int norm, const svbgpu_tensor *tensors, uint32_t ntensors, 
  * c is the factor of svbgpu_grad_clip from *d_norm and max_norm (d_norm == NULL: 1).  q saturates at the ends of
  * int32; an element whose e is infinite or NaN sends 0 and keeps its r.  The receiver calls svbgpu_decode_dequantize
  * with step.  d_residual_out may be d_residual; otherwise no two buffers overlap.  Bytes of d_out past the stream
- * are left as they were.  scale and 1 / scale are positive normal numbers.  Workspace as for svbgpu_encode. */
+ * are left as they were.  scale and 1 / scale are positive normal numbers.  Workspace as for svbgpu_encode.  The cache
+ * policy goes by the size alone: options "nt_threshold_mib" and "nt_force" do not apply. */
 int svbgpu_quantize_feedback_encode(int variant, int type, const void *d_grad, uint32_t count,
                                     const float *d_norm, double max_norm, float scale,
                                     const float *d_residual, float *d_residual_out, uint8_t *d_out,

@@ -259,8 +259,12 @@ class GradSet:
     def __init__(self, tensors, out=None):
         import torch
         from ._lib import GradTensor
+        tensors, outs = list(tensors), None if out is None else list(out)
+        for t in tensors + (outs or []):
+            if not isinstance(t, torch.Tensor):
+                raise ValueError(f"tensors, not {type(t).__name__}")
         tensors = [t.detach() for t in tensors]  # a later `t.data = ...` of the caller's does not reach these
-        outs = None if out is None else [t.detach() for t in out]
+        outs = None if outs is None else [t.detach() for t in outs]
         self.device = None
         for i, t in enumerate(tensors):
             self._look(t, f"tensor {i}")

@@ -138,6 +138,9 @@ def test_sets_look_their_tensors_over():
     with pytest.raises(ValueError, match="not a dense tensor on a device"):
         svb.GradSet([torch.zeros(3)])
     assert len(svb.GradSet([])) == 0
+    for wrong in ([None], [torch.zeros(3), 1.0], torch.zeros(2, 3).numpy()):  # a gradient that was never made
+        with pytest.raises(ValueError, match="tensors, not"):
+            svb.GradSet(wrong)
     with pytest.raises(ValueError, match="0 tensors, but 1 outputs"):
         svb.GradSet([], out=[torch.zeros(3)])
     from streamvbyte_amd import _dense, _grad_type
