@@ -228,12 +228,17 @@ def frame_decode_lists(frames):
 NORMS = {2: 2, 1: 1, float("inf"): 0}  # norm_type -> SVBGPU_NORM_*
 
 
+_GRAD_TYPES = {}  # torch type -> SVBGPU_F32 / _F16 / _BF16, filled on first use (torch is imported late)
+
+
 def _grad_type(torch, dtype):
     """SVBGPU_F32 / _F16 / _BF16 of a torch type; ValueError for any other."""
-    types = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-    if dtype not in types:
+    if not _GRAD_TYPES:
+        _GRAD_TYPES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    kind = _GRAD_TYPES.get(dtype)
+    if kind is None:
         raise ValueError(f"gradients are float32, float16 or bfloat16, not {dtype}")
-    return types[dtype]
+    return kind
 
 
 def _dense(t):
@@ -509,16 +514,17 @@ class DeviceCodec:
         if n > self.max_count:
             raise ValueError(f"{n} values, but the codec was made for {self.max_count}")
         residual_out = residual if residual_out is None else residual_out
-        for t, what in ((grad, "grad"), (residual, "residual"), (residual_out, "residual_out")):
-            if t.device != self.device or not t.is_contiguous() or t.numel() != n:
-                raise ValueError(f"{what}: a contiguous tensor of {n} elements on {self.device}")
+        device = self.device
+        for t in (grad, residual, residual_out):
+            if t.device != device or not t.is_contiguous() or t.numel() != n:
+                raise ValueError(f"grad, residual and residual_out are contiguous tensors of {n} elements on {device}")
         if residual.dtype != torch.float32 or residual_out.dtype != torch.float32:
             raise ValueError("the residual is float32")
         room = streamvbyte_max_compressedbytes(n)
         if out is None:
-            out = torch.empty(room, dtype=torch.uint8, device=self.device)
-        elif out.device != self.device or out.dtype != torch.uint8 or not out.is_contiguous() or out.numel() < room:
-            raise ValueError(f"out: a contiguous uint8 tensor of at least {room} bytes on {self.device}")
+            out = torch.empty(room, dtype=torch.uint8, device=device)
+        elif out.device != device or out.dtype != torch.uint8 or not out.is_contiguous() or out.numel() < room:
+            raise ValueError(f"out: a contiguous uint8 tensor of at least {room} bytes on {device}")
         if norm is not None:
             self._norm_word(norm, "norm")
         self._call("svbgpu_quantize_feedback_encode", variant, kind, grad.data_ptr(), n, None if norm is None else norm.data_ptr(),

@@ -389,6 +389,26 @@ def test_feedback_of_incompressible_gradients(torch, codec, oracle, variant):
     assert int(size.item()) == want.size == (n + 3) // 4 + 4 * n and np.array_equal(out[:want.size].cpu().numpy(), want)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("scale", [64.0, 7.3, 1e4])
+def test_feedback_against_64_bits(torch, codec, dtype, scale):
+    """What is sent plus what is left is what came in, g c + r, worked out in 64 bits.  Half a float32 step, h = 2^-24 of the
+    value, is lost at: the factor and the product (2 h |g c|), the sum e (h |e|), the step 1 / scale and the product
+    q step (2 h |q step|) and the difference (h |r'|); the scale itself is rounded once (h |q step|, as step is its
+    inverse).  And what is left is at most half a step: the product e scale is rounded before it is (h |e scale|)."""
+    h = 2.0 ** -24 * (1 + 2.0 ** -10)
+    for n in (5, 1027, 70001):
+        g, r = gradients(torch, n, dtype, seed=n + 7, far=100.0)
+        norm = torch.tensor([3.3], device="cuda")
+        out, size, new = codec.quantize_feedback_encode(g.cuda(), scale, r.cuda(), norm=norm, max_norm=1.1)
+        step = np.float32(1) / np.float32(scale)
+        sent, _ = codec.decode_dequantize(out, n, float(step))
+        gc = f64(g) * (1.1 / (f64(norm)[0] + 1e-6))
+        e, qs, left = gc + f64(r), f64(sent), f64(new)
+        assert (np.abs(qs + left - e) <= h * (2 * np.abs(gc) + np.abs(e) + 3 * np.abs(qs) + np.abs(left))).all()
+        assert (np.abs(left) <= 0.5 / scale + h * (4 * np.abs(e) + 4 * np.abs(qs) + 4 / scale)).all()
+
+
 def test_feedback_of_extremes(torch, codec, oracle):
     """Saturation at both ends of int32, infinities and NaN in gradient, residual and factor: such an element sends 0
     and keeps its residual; its neighbours do not notice."""
