@@ -16,7 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libstreamvbyte.so.2")
 LINK = os.path.join(HERE, "libstreamvbyte.so")
 # the same library with the look-back's stress hooks compiled in (csrc/svb_lookback.h: lb_stress_delay);
-# loaded only by tests/test_gpu_lookback_stress.py, through SVB_LIB_PATH
+# loaded only by the tests of it (test_gpu_lookback_stress.py, test_gpu_grad_stress.py), through SVB_LIB_PATH
 STRESS_LIB = os.path.join(HERE, "libstreamvbyte_stress.so.2")
 # No packed float32 arithmetic: some forms of v_pk_{add,mul,fma}_f32 have given wrong results now and then on these
 # cards, and the compiler makes them by itself from ordinary float code.  (The host pass does not know the feature and
@@ -25,7 +25,7 @@ DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 UNITS = ["svb_api", "svb_grad"]  # translation units: csrc/<unit>.hip
-OBJ = os.path.join(HERE, "build")
+OBJ = os.path.join(HERE, "obj")
 
 
 def with_includes(path, seen=None):
