@@ -26,6 +26,7 @@ inline hipStream_t S(void* s) { return reinterpret_cast<hipStream_t>(s); }
 constexpr u64 kCacheBytes = 256ull << 20;  // Infinity Cache
 constexpr u32 kNormMinChunk = 64 << 10;   // bytes of a norm's chunk ...
 constexpr u32 kNormChunks = 4096;         // ... which grows so that there are no more than this many, and one a tensor
+constexpr u64 kMaxSetBytes = (u64)kNormChunks << 31;  // a chunk's bytes fit 32 bits: what a workspace has words for
 constexpr u32 kMaxTensors = 1u << 22;     // so that a chunk's index in its launch fits 24 bits
 
 bool bad_type(int t) { return t != SVBGPU_F32 && t != SVBGPU_F16 && t != SVBGPU_BF16; }
@@ -48,6 +49,7 @@ int check_tensors(const svbgpu_tensor* t, uint32_t n, u64* total) {
     const u64 a = (u64)(uintptr_t)t[i].data;
     if (!a || (a & (b - 1)) || a >> kAddrBits || t[i].count >> (kCountBits - 3)) return SVBGPU_EINVAL;
     *total += t[i].count * b;
+    if (*total > kMaxSetBytes) return SVBGPU_EINVAL;
   }
   return SVBGPU_OK;
 }
@@ -133,9 +135,9 @@ int launch_small(const svbgpu_tensor* t, uint32_t n, void* const* outs, bool cli
 template <int KIND>
 int launch_norm(const svbgpu_tensor* t, uint32_t n, u64 total, u64 keep, float* d_norm, u64* partial, hipStream_t st) {
   u64 chunk = kNormMinChunk;
-  while (chunk * kNormChunks < total) chunk <<= 1;
+  while (chunk * kNormChunks < total) chunk <<= 1;  // 2^31 at most: check_tensors
   GradTable<kMaxSpans> table;
-  table.chunk_bytes = (u32)std::min<u64>(chunk, 1u << 31);
+  table.chunk_bytes = (u32)chunk;
   const u64 passing = total > keep ? total - keep : 0;  // bytes read to pass
   u64 bytes = 0;                                        // ... of the set that earlier launches read
   u32 before = 0;                                       // chunks of earlier launches
