@@ -258,10 +258,10 @@ int svbgpu_decode_dequantize(int variant, const uint8_t *d_in, float *d_out, uin
  * Gradient operators: what stands before and behind the two calls above in a training step.  No counterpart in the
  * reference.
  *
- * A call takes a host array of tensors (any number, of mixed types, in any order, each aligned to its element type,
- * empty ones allowed, 2^43 bytes in all at most); it is read before the call returns and travels in kernel arguments, so
- * a call can be captured into a graph and replayed.  Elements are counted as they lie in memory: a tensor is `count`
- * consecutive elements.
+ * A call takes a host array of tensors (of mixed types, in any order, each aligned to its element type, empty ones
+ * allowed; 2^31 tensors and 2^43 bytes in all at most); it is read before the call returns and travels in kernel
+ * arguments, so a call can be captured into a graph and replayed.  Elements are counted as they lie in memory: a tensor
+ * is `count` consecutive elements.
  * Workspace: svbgpu_grad_workspace_bytes(ntensors), 256-byte aligned, never initialised, for one call at a time.
  */
 #define SVBGPU_F32 0

@@ -27,7 +27,7 @@ constexpr u64 kCacheBytes = 256ull << 20;  // Infinity Cache
 constexpr u32 kNormMinChunk = 64 << 10;   // bytes of a norm's chunk ...
 constexpr u32 kNormChunks = 4096;         // ... which grows so that there are no more than this many, and one a tensor
 constexpr u64 kMaxSetBytes = (u64)kNormChunks << 31;  // a chunk's bytes fit 32 bits: what a workspace has words for
-constexpr u32 kMaxTensors = 1u << 22;     // so that a chunk's index in its launch fits 24 bits
+constexpr u32 kMaxTensors = 1u << 31;     // with it the chunks of all launches fit 32 bits
 
 bool bad_type(int t) { return t != SVBGPU_F32 && t != SVBGPU_F16 && t != SVBGPU_BF16; }
 bool bad_norm(int n) { return n != SVBGPU_NORM_MAX && n != SVBGPU_NORM_L1 && n != SVBGPU_NORM_L2; }

@@ -23,3 +23,23 @@ def test_bytes_of_a_set():
     room = [(A, longest, F32)] * 15 + [(A, 16, F32)] * 1000                  # more tensors, fewer bytes
     assert norm(room) == ENODEVICE
     assert clip([(1 << 40, longest, F32)], given=1) == ENODEVICE
+
+
+def test_any_number_of_tensors():
+    """Chunks are counted anew in every launch, so the number of tensors is bounded by the 32 bits of all chunks alone."""
+    import ctypes as C
+    from streamvbyte_amd._lib import GradTensor
+    lib = svb.load()
+    n = (1 << 22) + 1
+    table = (GradTensor * n)()  # all empty
+    for i in (0, n // 2, n - 1):
+        table[i] = GradTensor(A + 4096 * i, 3, F32)
+    room = lib.svbgpu_grad_workspace_bytes(n)
+    assert room >= 8 * (4096 + n)
+    ws = 0x7000_0000_0000
+    assert lib.svbgpu_grad_norm(2, table, n, 0x1000, ws, room, None) == ENODEVICE
+    assert lib.svbgpu_grad_norm(2, table, n, 0x1000, ws, room - 256, None) == -3
+    assert lib.svbgpu_grad_clip(2, table, n, None, 1.0, 0, 0x1000, ws, room, None) == ENODEVICE
+    # beyond the limit the table is not even read
+    assert lib.svbgpu_grad_norm(2, C.c_void_p(1 << 12), (1 << 31) + 1, 0x1000, ws, 1 << 40, None) == EINVAL
+    assert lib.svbgpu_grad_workspace_bytes((1 << 32) - 1) >= 8 * (4096 + (1 << 32) - 1)
