@@ -488,17 +488,18 @@ class DeviceCodec:
     def clip_grads(self, grads, max_norm, norm_type=2.0, norm=None):
         """Multiplies every element of `grads` (a GradSet or a list of tensors) by min(1, max_norm / (N + 1e-6)), N their
         global norm, in place or into the GradSet's `out` tensors; returns N, a float32 tensor[1].  `norm`: N worked out
-        before (over other ranks' shards too, say); it is then read instead, and returned."""
-        if norm_type not in NORMS:
+        before (over other ranks' shards too, say); it is then read instead, and returned, and norm_type is not looked at."""
+        given = norm is not None
+        kind = 2 if given else NORMS.get(norm_type)
+        if kind is None:
             raise ValueError(f"norm_type {norm_type}: 1, 2 or inf")
         if not max_norm >= 0:
             raise ValueError(f"max_norm {max_norm}")
         grads = grads if isinstance(grads, GradSet) else GradSet(grads)
         grads._check(self.device)
-        given = norm is not None
         norm = self._norm_word(norm, "norm") if given else self.torch.empty(1, dtype=self.torch.float32, device=self.device)
         ws = self._grad_workspace(len(grads))
-        self._call("svbgpu_grad_clip", NORMS[norm_type], grads.table, len(grads), grads.out_table, max_norm, int(given),
+        self._call("svbgpu_grad_clip", kind, grads.table, len(grads), grads.out_table, max_norm, int(given),
                    norm.data_ptr(), ws.data_ptr(), ws.numel())
         return norm
 

@@ -255,7 +255,7 @@ int svbgpu_grad_norm(int norm, const svbgpu_tensor* tensors, uint32_t ntensors, 
 int svbgpu_grad_clip(int norm, const svbgpu_tensor* tensors, uint32_t ntensors, void* const* outs, double max_norm, int norm_given,
                      float* d_norm, void* ws, size_t ws_bytes, void* stream) {
   u64 total;
-  if (bad_norm(norm) || !d_norm || ((uintptr_t)d_norm & 3u) || !(max_norm >= 0.0)) return SVBGPU_EINVAL;
+  if ((!norm_given && bad_norm(norm)) || !d_norm || ((uintptr_t)d_norm & 3u) || !(max_norm >= 0.0)) return SVBGPU_EINVAL;
   int rc = check_tensors(tensors, ntensors, &total);
   if (!rc) rc = check_written(tensors, ntensors, outs);
   if (rc) return rc;

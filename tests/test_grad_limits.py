@@ -43,3 +43,10 @@ def test_any_number_of_tensors():
     # beyond the limit the table is not even read
     assert lib.svbgpu_grad_norm(2, C.c_void_p(1 << 12), (1 << 31) + 1, 0x1000, ws, 1 << 40, None) == EINVAL
     assert lib.svbgpu_grad_workspace_bytes((1 << 32) - 1) >= 8 * (4096 + (1 << 32) - 1)
+
+
+def test_a_given_norm_needs_no_kind_and_no_workspace():
+    rows = [(A, 10, F32)]
+    for kind in (2, 1, 0, 3, -1):
+        assert clip(rows, kind=kind, ws=None, given=1) == ENODEVICE, kind
+    assert clip(rows, kind=3) == EINVAL and clip(rows, kind=-1) == EINVAL
