@@ -290,8 +290,9 @@ class GradSet:
         self.table = (GradTensor * max(n, 1))(*[GradTensor(t.data_ptr() or None, t.numel(), _grad_type(torch, t.dtype))
                                                 for t in self.tensors])
         self.out_table = None if outs is None else (C.c_void_p * max(n, 1))(*[t.data_ptr() or None for t in self.outs])
-        # a tensor keeps its place in its storage, so one tensor a storage tells whether any has moved
-        self._held = list({t.untyped_storage().data_ptr(): t for t in self.tensors + (self.outs or [])}.values())
+        # a tensor keeps its place in its storage, so one tensor a storage tells whether any has moved (an empty one has
+        # no address)
+        self._held = list({t.untyped_storage().data_ptr(): t for t in self.tensors + (self.outs or []) if t.numel()}.values())
         self._addresses = [t.data_ptr() for t in self._held]
         self._indices = list(range(len(self._held)))
         self._compare = getattr(torch._C, "_tensors_data_ptrs_at_indices_equal", None)

@@ -43,3 +43,34 @@ def test_a_given_norm_is_of_any_kind(codec):
         codec.clip_grads(x, 1.0, norm_type=p, norm=given)
         codec.clip_grads(x, 1.0, norm_type=p)
     assert len(codec.calls) == 7
+
+
+def moved(codec, grads, owner):
+    """Whether the set is refused once `owner`'s storage has given its memory back."""
+    codec.grad_norm(grads)
+    owner.untyped_storage().resize_(0)
+    try:
+        codec.grad_norm(grads)
+    except ValueError as e:
+        assert "moved" in str(e)
+        return True
+    return False
+
+
+def test_memory_given_back_is_noticed(codec):
+    """One tensor a storage is compared; an empty one has no address that could tell.  (The results are compared by
+    themselves: a failed assert would print tensors that have no memory any more.)"""
+    def buffers():
+        return torch.randn(100), torch.randn(100)
+    seen = {}
+    x, _ = buffers()
+    seen["two views"] = moved(codec, svb.GradSet([dev(x[:40]), dev(x[40:])]), x)
+    x, _ = buffers()
+    seen["empty views beside it"] = moved(codec, svb.GradSet([dev(x[:0]), dev(x), dev(x[7:7])]), x)
+    x, y = buffers()
+    seen["an empty output in an input's storage"] = moved(codec, svb.GradSet([dev(x), dev(y[:0])], out=[dev(y), dev(x[:0])]), x)
+    x, y = buffers()
+    seen["and the other way round"] = moved(codec, svb.GradSet([dev(x), dev(y[:0])], out=[dev(y), dev(x[:0])]), y)
+    x, y = buffers()
+    seen["another tensor's"] = not moved(codec, svb.GradSet([dev(x), dev(x[:0])]), y)
+    assert seen == dict.fromkeys(seen, True)
