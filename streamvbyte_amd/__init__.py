@@ -225,6 +225,13 @@ def frame_decode_lists(frames):
 
 
 # ---- gradient tensors -----------------------------------------------------------
+def _count_written(torch, tensors):
+    """Counts on the versions of tensors that the library has written, as in-place operations of torch's do: a graph that
+    saved one then refuses its backward pass."""
+    count = getattr(torch._C, "_increment_version", None) or torch.autograd.graph.increment_version
+    count(tensors)
+
+
 NORMS = {2: 2, 1: 1, float("inf"): 0}  # norm_type -> SVBGPU_NORM_*
 
 
@@ -268,6 +275,8 @@ class GradSet:
         for t in tensors + (outs or []):
             if not isinstance(t, torch.Tensor):
                 raise ValueError(f"tensors, not {type(t).__name__}")
+        # what a clip writes: tensors whose versions it counts on.  Views share their base's version.
+        written = None if outs is None else list({t if t._base is None else t._base: t for t in outs}.values())
         tensors = [t.detach() for t in tensors]  # a later `t.data = ...` of the caller's does not reach these
         outs = None if outs is None else [t.detach() for t in outs]
         self.device = None
@@ -296,6 +305,7 @@ class GradSet:
         self._addresses = [t.data_ptr() for t in self._held]
         self._indices = list(range(len(self._held)))
         self._compare = getattr(torch._C, "_tensors_data_ptrs_at_indices_equal", None)
+        self.written = self.tensors if written is None else [t.detach() for t in written]
 
     def _look(self, t, what):
         if not t.is_cuda or str(t.layout) != "torch.strided":
@@ -484,6 +494,8 @@ class DeviceCodec:
         norm = self.torch.empty(1, dtype=self.torch.float32, device=self.device) if out is None else self._norm_word(out, "out")
         ws = self._grad_workspace(len(grads))
         self._call("svbgpu_grad_norm", NORMS[norm_type], grads.table, len(grads), norm.data_ptr(), ws.data_ptr(), ws.numel())
+        if out is not None:
+            _count_written(self.torch, [out])
         return norm
 
     def clip_grads(self, grads, max_norm, norm_type=2.0, norm=None):
@@ -502,6 +514,7 @@ class DeviceCodec:
         ws = self._grad_workspace(len(grads))
         self._call("svbgpu_grad_clip", kind, grads.table, len(grads), grads.out_table, max_norm, int(given),
                    norm.data_ptr(), ws.data_ptr(), ws.numel())
+        _count_written(self.torch, grads.written)
         return norm
 
     def quantize_feedback_encode(self, grad, scale, residual, norm=None, max_norm=float("inf"), out=None, residual_out=None,
@@ -523,15 +536,19 @@ class DeviceCodec:
         if residual.dtype != torch.float32 or residual_out.dtype != torch.float32:
             raise ValueError("the residual is float32")
         room = streamvbyte_max_compressedbytes(n)
+        written = [residual_out]
         if out is None:
             out = torch.empty(room, dtype=torch.uint8, device=device)
         elif out.device != device or out.dtype != torch.uint8 or not out.is_contiguous() or out.numel() < room:
             raise ValueError(f"out: a contiguous uint8 tensor of at least {room} bytes on {device}")
+        else:
+            written.append(out)
         if norm is not None:
             self._norm_word(norm, "norm")
         self._call("svbgpu_quantize_feedback_encode", variant, kind, grad.data_ptr(), n, None if norm is None else norm.data_ptr(),
                    max_norm, scale, residual.data_ptr(), residual_out.data_ptr(), out.data_ptr(), self.ws.data_ptr(),
                    self.ws_bytes, self._res_ptr(0))
+        _count_written(torch, written)
         return out, self.res[0:1], residual_out
 
     def decode_intersect(self, stream, count, sorted_values, out=None, variant=V1234, prev=0):

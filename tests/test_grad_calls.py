@@ -74,3 +74,71 @@ def test_memory_given_back_is_noticed(codec):
     x, y = buffers()
     seen["another tensor's"] = not moved(codec, svb.GradSet([dev(x), dev(x[:0])]), y)
     assert seen == dict.fromkeys(seen, True)
+
+
+def versions(*tensors):
+    return [t._version for t in tensors]
+
+
+def test_what_is_written_counts_as_written(codec):
+    """The library writes behind torch's back: every tensor of the caller's that a call writes has its version counted on,
+    so that a graph that saved one refuses its backward pass, as after an in-place operation of torch's own."""
+    a, b = torch.randn(10), torch.randn(3, 3)
+    grads = [dev(a), dev(b)]
+    was = versions(a, b)
+    codec.grad_norm(grads)
+    assert versions(a, b) == was                    # only read
+    codec.clip_grads(grads, 1.0)
+    assert all(v > w for v, w in zip(versions(a, b), was))
+    was = versions(a, b)
+    outs = [torch.empty(10), torch.empty(3, 3)]
+    outs_were = versions(*outs)
+    codec.clip_grads(svb.GradSet(grads, out=[dev(t) for t in outs]), 1.0)
+    assert versions(a, b) == was and all(v > w for v, w in zip(versions(*outs), outs_were))
+    # views of one bucket
+    bucket = torch.randn(100)
+    kept = svb.GradSet([dev(t) for t in bucket.split(10)])
+    spare = svb.GradSet([dev(t) for t in torch.randn(100).split(10)], out=[dev(t) for t in bucket.split(10)])
+    for s in (kept, spare):
+        for _ in range(2):
+            was = bucket._version
+            codec.clip_grads(s, 1.0)
+            assert bucket._version > was
+    # norms and residuals
+    word = torch.zeros(1)
+    codec.grad_norm(grads, out=word)
+    assert word._version == 1
+    codec.clip_grads(grads, 1.0, norm=word)
+    assert word._version == 1                       # only read
+    g, r, new, out = torch.randn(8), torch.zeros(8), torch.zeros(8), torch.zeros(100, dtype=torch.uint8)
+    codec.quantize_feedback_encode(g, 4.0, r, norm=word)
+    assert versions(g, r, word) == [0, 1, 1]
+    codec.quantize_feedback_encode(g, 4.0, r, out=out, residual_out=new)
+    assert versions(g, r, new, out) == [0, 1, 1, 1]
+
+
+def test_a_saved_gradient_is_not_changed_unseen(codec):
+    w = torch.randn(6, requires_grad=True)
+    for change in (lambda g: codec.clip_grads([dev(g)], 1.0),
+                   lambda g: codec.clip_grads(svb.GradSet([dev(torch.ones(6))], out=[dev(g)]), 1.0),
+                   lambda g: codec.quantize_feedback_encode(torch.ones(6), 4.0, g)):
+        g = torch.randn(6)
+        loss = (w * g).sum()
+        change(g)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+
+
+def test_tensors_without_versions(codec):
+    """Tensors made in inference mode have none; ordinary ones have theirs there too."""
+    with torch.inference_mode():
+        a, r = torch.randn(10), torch.zeros(10)
+        for _ in range(2):
+            codec.clip_grads([dev(a)], 1.0)
+            codec.quantize_feedback_encode(a, 4.0, r)
+    codec.clip_grads([dev(a)], 1.0)
+    codec.quantize_feedback_encode(a, 4.0, r)
+    b = torch.randn(10)
+    with torch.inference_mode():
+        codec.clip_grads([dev(b)], 1.0)
+    assert b._version == 1 and len(codec.calls) == 7
