@@ -314,6 +314,8 @@ class GradSet:
             self.device = t.device
         elif t.device != self.device:
             raise ValueError(f"{what} is on {t.device}, the first on {self.device}")
+        if t.is_neg():
+            raise ValueError(f"{what} is negated lazily: pass its resolve_neg()")
         if not _dense(t):
             raise ValueError(f"{what} has gaps or repeats in its memory: strides {t.stride()} of shape {tuple(t.shape)}")
 
@@ -481,6 +483,8 @@ class DeviceCodec:
     def _norm_word(self, t, what):
         if not (t.device == self.device and t.dtype == self.torch.float32 and t.numel() == 1):
             raise ValueError(f"{what}: a one-element float32 tensor on {self.device}")
+        if t.is_neg():
+            raise ValueError(f"{what} is negated lazily: pass its resolve_neg()")
         return t
 
     def grad_norm(self, grads, norm_type=2.0, out=None):
@@ -533,6 +537,8 @@ class DeviceCodec:
         for t in (grad, residual, residual_out):
             if t.device != device or not t.is_contiguous() or t.numel() != n:
                 raise ValueError(f"grad, residual and residual_out are contiguous tensors of {n} elements on {device}")
+            if t.is_neg():
+                raise ValueError("a tensor is negated lazily: pass its resolve_neg()")
         if residual.dtype != torch.float32 or residual_out.dtype != torch.float32:
             raise ValueError("the residual is float32")
         room = streamvbyte_max_compressedbytes(n)

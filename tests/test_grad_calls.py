@@ -142,3 +142,27 @@ def test_tensors_without_versions(codec):
     with torch.inference_mode():
         codec.clip_grads([dev(b)], 1.0)
     assert b._version == 1 and len(codec.calls) == 7
+
+
+def test_lazily_negated_tensors_are_refused(codec):
+    """What such a tensor's memory holds is not its values."""
+    z = torch.complex(torch.tensor([1.0]), torch.tensor([2.0]))
+    x = z.conj().imag                               # -2, of which memory holds 2
+    assert x.is_neg() and x.is_contiguous() and float(x) == -2.0
+    plain = torch.zeros(1)
+    for wrong in (lambda: svb.GradSet([dev(x)]), lambda: svb.GradSet([dev(plain)], out=[dev(x)]),
+                  lambda: svb.GradSet([dev(plain), dev(x)])):
+        with pytest.raises(ValueError, match="negated"):
+            wrong()
+    for change in (dict(grad=x), dict(residual=x), dict(residual_out=x)):
+        with pytest.raises(ValueError, match="negated"):
+            codec.quantize_feedback_encode(**dict(dict(grad=plain, scale=4.0, residual=torch.zeros(1)), **change))
+    with pytest.raises(ValueError, match="negated"):
+        codec.grad_norm([dev(plain)], out=x)
+    with pytest.raises(ValueError, match="negated"):
+        codec.clip_grads([dev(plain)], 1.0, norm=x)
+    assert not codec.calls
+    y = x.resolve_neg()
+    codec.grad_norm([dev(y)])
+    codec.quantize_feedback_encode(y, 4.0, plain)
+    assert len(codec.calls) == 2
