@@ -1,6 +1,7 @@
 """Build libstreamvbyte.so.2 (HIP, gfx950) in-tree.
 
     python -m streamvbyte_amd.build [--force]
+    python -m streamvbyte_amd.build --variant OUT [hipcc flags]
 
 The translation units of csrc/ side by side, then one link; the library lands next to this file
 so that it travels with the source tree.
@@ -22,7 +23,7 @@ STRESS_LIB = os.path.join(HERE, "libstreamvbyte_stress.so.2")
 # cards, and the compiler makes them by itself from ordinary float code.  (The host pass does not know the feature and
 # says so: harmless.)
 DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", *DEVICE_FLAGS]
 
 UNITS = ["svb_api", "svb_grad"]  # translation units: csrc/<unit>.hip
 OBJ = os.path.join(HERE, "obj")
@@ -60,22 +61,29 @@ def _wait(jobs):
             raise subprocess.CalledProcessError(rc, args)
 
 
+def _compiles(extra, tag):
+    """(object, its dependencies, the command that makes it) of every unit."""
+    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+    out = []
+    for unit in UNITS:
+        src, obj = os.path.join(CSRC, unit + ".hip"), os.path.join(OBJ, unit + tag + ".o")
+        out.append((obj, with_includes(src), [hipcc, *FLAGS, "-fPIC", "-Wall", "-Wno-unused-function", *extra,
+                                              "-I", os.path.join(ROOT, "include"), "-c", src, "-o", obj]))
+    return out
+
+
+def _link(lib, objects):
+    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+    return [hipcc, "--offload-arch=gfx950", "-fPIC", "-shared", "-Wl,-soname,libstreamvbyte.so.2", "-o", lib, *objects, "-ldl"]
+
+
 def build(force=False, verbose=True):
     """Both libraries: every stale unit compiled side by side, then linked."""
-    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     os.makedirs(OBJ, exist_ok=True)
-    objects = {LIB: [], STRESS_LIB: []}
-    jobs = []
-    for lib, extra, tag in ((LIB, [], ""), (STRESS_LIB, ["-DSVB_LB_STRESS"], ".stress")):
-        for unit in UNITS:
-            src, obj = os.path.join(CSRC, unit + ".hip"), os.path.join(OBJ, unit + tag + ".o")
-            objects[lib].append(obj)
-            if force or stale(obj, with_includes(src)):
-                jobs.append(_run([hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
-                                  *DEVICE_FLAGS, *extra, "-I", os.path.join(ROOT, "include"), "-c", src, "-o", obj], verbose))
-    _wait(jobs)
-    jobs = [_run([hipcc, "--offload-arch=gfx950", "-fPIC", "-shared", "-Wl,-soname,libstreamvbyte.so.2", "-o", lib, *objs, "-ldl"], verbose)
-            for lib, objs in objects.items() if force or stale(lib, objs)]
+    plans = [(LIB, _compiles([], "")), (STRESS_LIB, _compiles(["-DSVB_LB_STRESS"], ".stress"))]
+    _wait([_run(cmd, verbose) for _, units in plans for obj, deps, cmd in units if force or stale(obj, deps)])
+    jobs = [_run(_link(lib, [obj for obj, *_ in units]), verbose) for lib, units in plans
+            if force or stale(lib, [obj for obj, *_ in units])]
     _wait(jobs)
     if jobs:
         if os.path.lexists(LINK):
@@ -84,5 +92,17 @@ def build(force=False, verbose=True):
     return LIB
 
 
+def build_variant(out, extra, verbose=True):
+    """The library with extra compiler flags, as `out`: for A/B comparisons through SVB_LIB_PATH."""
+    os.makedirs(OBJ, exist_ok=True)
+    units = _compiles(list(extra), "." + os.path.basename(out))
+    _wait([_run(cmd, verbose) for *_, cmd in units])
+    _wait([_run(_link(out, [obj for obj, *_ in units]), verbose)])
+
+
 if __name__ == "__main__":
-    build(force="--force" in sys.argv)
+    if "--variant" in sys.argv:
+        at = sys.argv.index("--variant")
+        build_variant(os.path.abspath(sys.argv[at + 1]), sys.argv[at + 2:])
+    else:
+        build(force="--force" in sys.argv)

@@ -8,8 +8,7 @@ set -e -o pipefail
 ROOT=$(cd "$(dirname "$0")/.." && pwd)
 ALT=$ROOT/streamvbyte_amd/libstreamvbyte_lds_table.so
 if [ "$1" = build ]; then
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -shared -DSVB_LENGTH_TABLE_LDS -Wl,-soname,libstreamvbyte.so.2 \
-      -I "$ROOT/include" -o "$ALT" "$ROOT/streamvbyte_amd/csrc/svb_api.hip"
+  cd "$ROOT" && python3 -m streamvbyte_amd.build --variant "$ALT" -DSVB_LENGTH_TABLE_LDS
   echo "built $ALT"
 else
   for i in 1 2 3; do

@@ -9,9 +9,10 @@ args = sys.argv[1:]
 unit = "svb_api"
 if args[:1] == ["--unit"]:
     unit, args = args[1], args[2:]
-cmd = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + args + [ "-I", os.path.join(ROOT, "include"),
-       "--cuda-device-only", "-c", "-Rpass-analysis=kernel-resource-usage", "-o", "/dev/null",
-       os.path.join(ROOT, f"streamvbyte_amd/csrc/{unit}.hip")]
+sys.path.insert(0, ROOT)
+from streamvbyte_amd.build import CSRC, FLAGS
+cmd = ["/opt/rocm/bin/hipcc", *FLAGS, *args, "-I", os.path.join(ROOT, "include"), "--cuda-device-only", "-c",
+       "-Rpass-analysis=kernel-resource-usage", "-o", "/dev/null", os.path.join(CSRC, unit + ".hip")]
 out = subprocess.run(cmd, capture_output=True, text=True).stderr
 cur = {}
 rows = []
