@@ -78,14 +78,14 @@ def _link(lib, objects):
 
 
 def build(force=False, verbose=True):
-    """Both libraries: every stale unit compiled side by side, then linked."""
+    """Both libraries, where a source is newer: every stale unit compiled side by side, then linked."""
     os.makedirs(OBJ, exist_ok=True)
     plans = [(LIB, _compiles([], "")), (STRESS_LIB, _compiles(["-DSVB_LB_STRESS"], ".stress"))]
+    if not force:  # by the sources alone: a built tree may have been copied without its objects
+        plans = [(lib, units) for lib, units in plans if any(stale(lib, deps) for _, deps, _ in units)]
     _wait([_run(cmd, verbose) for _, units in plans for obj, deps, cmd in units if force or stale(obj, deps)])
-    jobs = [_run(_link(lib, [obj for obj, *_ in units]), verbose) for lib, units in plans
-            if force or stale(lib, [obj for obj, *_ in units])]
-    _wait(jobs)
-    if jobs:
+    _wait([_run(_link(lib, [obj for obj, *_ in units]), verbose) for lib, units in plans])
+    if plans:
         if os.path.lexists(LINK):
             os.remove(LINK)
         os.symlink(os.path.basename(LIB), LINK)

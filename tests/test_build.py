@@ -61,3 +61,32 @@ def test_tools_compile_through_the_build():
     text = open(os.path.join(tools, "ab_length_table.sh")).read()
     assert "streamvbyte_amd.build --variant" in text and "-DSVB_LENGTH_TABLE_LDS" in text
     subprocess.check_call(["bash", "-n", os.path.join(tools, "ab_length_table.sh")])
+
+
+def test_only_what_is_out_of_date_is_made(recorder):
+    b.build(verbose=False)
+    assert sorted(recorder.units()) == sorted(2 * HIP) and os.readlink(b.LINK) == os.path.basename(b.LIB)
+    later = max(os.path.getmtime(p) for p in (b.LIB, b.STRESS_LIB)) + 10
+
+    def commands(force=False):
+        recorder.commands.clear()
+        b.build(force=force, verbose=False)
+        return len(recorder.commands)
+    assert commands() == 0
+    # libraries that travelled without their objects are as good as they were
+    for f in os.listdir(b.OBJ):
+        os.remove(os.path.join(b.OBJ, f))
+    assert commands() == 0
+    # ... until a library is missing or older than a source, or everything is asked for
+    os.remove(b.STRESS_LIB)
+    assert commands() == len(HIP) + 1
+    for f in os.listdir(b.OBJ):
+        os.utime(os.path.join(b.OBJ, f), (0, 0))
+    os.utime(b.LIB, (0, 0))
+    assert commands() == len(HIP) + 1
+    # a link that did not happen is made up for
+    for f in os.listdir(b.OBJ):
+        os.utime(os.path.join(b.OBJ, f), (later, later))
+    os.utime(b.LIB, (0, 0))
+    assert commands() == 1
+    assert commands(force=True) == 2 * len(HIP) + 2
