@@ -202,16 +202,18 @@ int run(int kind, const svbgpu_tensor* t, uint32_t n, u64 total, void* const* ou
   return run_kind<kNormEuclid>(t, n, total, outs, clip, limit, d_norm, ws, st);
 }
 
-template <int V, int T, int QW, bool DEFER, int NT>
-void launch_feedback(u32 nw, const void* grad, uint32_t count, uint8_t* d_out, const FeedArgs& fa, void* ws, unsigned tag2,
+template <int V, int T, int QW, bool DEFER, int NT, u32 NW>
+void launch_feedback(const void* grad, uint32_t count, uint8_t* d_out, const FeedArgs& fa, void* ws, unsigned tag2,
                      uint64_t* d_written, hipStream_t st) {
-  const WsLayout L = ws_layout(count);  // has a look-back word per kWaves wave tiles: nw * QW >= kWaves
-  const u32 tile = nw * QW * kWtInts, tiles = (u32)(((u64)count + tile - 1) / tile);
+  static_assert(NW * QW >= kWaves, "the workspace has a look-back word per kWaves wave tiles");
+  static_assert(NW <= kFeedMaxWaves, "the kernel's LDS holds that many waves' images");
+  const WsLayout L = ws_layout(count);
+  const u32 tile = NW * QW * kWtInts, tiles = (u32)(((u64)count + tile - 1) / tile);
   const u32 grid = std::min<u32>(tiles, (u32)std::max(host::device_cus(), 1));
   WsHeader* h = reinterpret_cast<WsHeader*>(static_cast<char*>(ws) + ((tag2 >> 3) & 1u) * 8);
   const LbWords lb{reinterpret_cast<u64*>(static_cast<char*>(ws) + L.off_status), (u32)((L.off_lb_group - L.off_status) / 8), tag2};
-  hipLaunchKernelGGL((k_feedback_encode<V, T, QW, DEFER, NT>), dim3(grid), dim3((nw + 1) * 64), 0, st, static_cast<const u8*>(grad), count,
-                     tiles, nw, d_out, fa, h, lb, d_written);
+  hipLaunchKernelGGL((k_feedback_encode<V, T, QW, DEFER, NT>), dim3(grid), dim3((NW + 1) * 64), 0, st, static_cast<const u8*>(grad), count,
+                     tiles, NW, d_out, fa, h, lb, d_written);
 }
 // The tile by size.  A large tile means few look-backs, a small one that a short stream reaches more of the device; the
 // deferred copy hides the look-backs where a workgroup takes several tiles.  Measured with float32, 0124, us for QW x nw
@@ -229,11 +231,14 @@ template <int V, int T>
 void launch_feedback(const void* grad, uint32_t count, uint8_t* d_out, const FeedArgs& fa, void* ws, unsigned tag2, uint64_t* d_written,
                      hipStream_t st) {
   const u32 m = count >> 19;  // in half millions
-  if (m < 3) launch_feedback<V, T, 1, false, 0>(m < 1 ? 4 : 8, grad, count, d_out, fa, ws, tag2, d_written, st);
-  else if (m < 7) launch_feedback<V, T, 1, false, 0>(15, grad, count, d_out, fa, ws, tag2, d_written, st);
-  else if (m < 15) launch_feedback<V, T, 2, false, kNtStores>(m < 12 ? 12 : 15, grad, count, d_out, fa, ws, tag2, d_written, st);
-  else if (m < 32) launch_feedback<V, T, 1, true, kNtStores>(15, grad, count, d_out, fa, ws, tag2, d_written, st);
-  else launch_feedback<V, T, 1, true, kNtLoads | kNtStores>(15, grad, count, d_out, fa, ws, tag2, d_written, st);
+  const auto go = [&](auto launch) { launch(grad, count, d_out, fa, ws, tag2, d_written, st); };
+  if (m < 1) go(launch_feedback<V, T, 1, false, 0, 4>);
+  else if (m < 3) go(launch_feedback<V, T, 1, false, 0, 8>);
+  else if (m < 7) go(launch_feedback<V, T, 1, false, 0, 15>);
+  else if (m < 12) go(launch_feedback<V, T, 2, false, kNtStores, 12>);
+  else if (m < 15) go(launch_feedback<V, T, 2, false, kNtStores, 15>);
+  else if (m < 32) go(launch_feedback<V, T, 1, true, kNtStores, 15>);
+  else go(launch_feedback<V, T, 1, true, kNtLoads | kNtStores, 15>);
 }
 
 }  // namespace
