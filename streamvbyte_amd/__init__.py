@@ -228,8 +228,7 @@ def frame_decode_lists(frames):
 def _count_written(torch, tensors):
     """Counts on the versions of tensors that the library has written, as in-place operations of torch's do: a graph that
     saved one then refuses its backward pass."""
-    count = getattr(torch._C, "_increment_version", None) or torch.autograd.graph.increment_version
-    count(tensors)
+    torch._C._increment_version(tensors)
 
 
 NORMS = {2: 2, 1: 1, float("inf"): 0}  # norm_type -> SVBGPU_NORM_*
@@ -268,6 +267,8 @@ class GradSet:
     gradients keep their memory from step to step makes one GradSet and passes it to every call; it holds the
     tensors, and raises if one of them has moved since.  Passing a plain list makes one on the spot."""
 
+    _kept = True  # made by the caller, for many calls
+
     def __init__(self, tensors, out=None):
         import torch
         from ._lib import GradTensor
@@ -275,47 +276,50 @@ class GradSet:
         for t in tensors + (outs or []):
             if not isinstance(t, torch.Tensor):
                 raise ValueError(f"tensors, not {type(t).__name__}")
-        # what a clip writes: tensors whose versions it counts on.  Views share their base's version.
-        written = None if outs is None else list({t if t._base is None else t._base: t for t in outs}.values())
+        # what a clip writes: tensors whose versions it counts on
+        self.written = tensors if outs is None else outs
+        if self._kept:  # views share their base's version, tensors of inference mode have none
+            self.written = [t.detach() for t in {t if t._base is None else t._base: t for t in self.written}.values() if not t.is_inference()]
         tensors = [t.detach() for t in tensors]  # a later `t.data = ...` of the caller's does not reach these
         outs = None if outs is None else [t.detach() for t in outs]
         self.device = None
         for i, t in enumerate(tensors):
-            self._look(t, f"tensor {i}")
+            self._look(torch, t, f"tensor {i}")
         if outs is not None:
             if len(outs) != len(tensors):
                 raise ValueError(f"{len(tensors)} tensors, but {len(outs)} outputs")
             for i, (t, y) in enumerate(zip(tensors, outs)):
-                self._look(y, f"output {i}")
+                self._look(torch, y, f"output {i}")
                 same_layout = y.stride() == t.stride() or (y.is_contiguous() and t.is_contiguous())
                 if y.dtype != t.dtype or y.shape != t.shape or not same_layout:
                     raise ValueError(f"output {i} is not of its tensor's type, shape and strides")
         # in the order of the memory that a clip writes, in which the library checks it fastest
-        written = tensors if outs is None else outs
-        order = sorted(range(len(tensors)), key=lambda i: written[i].data_ptr())
+        places = [t.data_ptr() for t in (tensors if outs is None else outs)]
+        order = sorted(range(len(tensors)), key=places.__getitem__)
         self.tensors = [tensors[i] for i in order]
         self.outs = None if outs is None else [outs[i] for i in order]
         n = len(tensors)
-        self.table = (GradTensor * max(n, 1))(*[GradTensor(t.data_ptr() or None, t.numel(), _grad_type(torch, t.dtype))
-                                                for t in self.tensors])
+        counts = [t.numel() for t in self.tensors]
+        if 1 in counts and any(t.is_neg() for t in self.tensors + (self.outs or [])):  # larger ones are not dense
+            raise ValueError("a tensor is negated lazily: pass its resolve_neg()")
+        self.table = (GradTensor * max(n, 1))(*[GradTensor(t.data_ptr() or None, c, _grad_type(torch, t.dtype))
+                                                for t, c in zip(self.tensors, counts)])
         self.out_table = None if outs is None else (C.c_void_p * max(n, 1))(*[t.data_ptr() or None for t in self.outs])
         # a tensor keeps its place in its storage, so one tensor a storage tells whether any has moved (an empty one has
         # no address)
-        self._held = list({t.untyped_storage().data_ptr(): t for t in self.tensors + (self.outs or []) if t.numel()}.values())
+        self._held = list({t.untyped_storage().data_ptr(): t
+                           for s in (self.tensors, self.outs or []) for t, c in zip(s, counts) if c}.values())
         self._addresses = [t.data_ptr() for t in self._held]
         self._indices = list(range(len(self._held)))
         self._compare = getattr(torch._C, "_tensors_data_ptrs_at_indices_equal", None)
-        self.written = self.tensors if written is None else [t.detach() for t in written]
 
-    def _look(self, t, what):
-        if not t.is_cuda or str(t.layout) != "torch.strided":
+    def _look(self, torch, t, what):
+        if not t.is_cuda or t.layout is not torch.strided:
             raise ValueError(f"{what} is not a dense tensor on a device")
         if self.device is None:
             self.device = t.device
         elif t.device != self.device:
             raise ValueError(f"{what} is on {t.device}, the first on {self.device}")
-        if t.is_neg():
-            raise ValueError(f"{what} is negated lazily: pass its resolve_neg()")
         if not _dense(t):
             raise ValueError(f"{what} has gaps or repeats in its memory: strides {t.stride()} of shape {tuple(t.shape)}")
 
@@ -331,6 +335,11 @@ class GradSet:
 
     def __len__(self):
         return len(self.tensors)
+
+
+class _OneCallSet(GradSet):
+    """What a plain list becomes."""
+    _kept = False
 
 
 class DeviceCodec:
@@ -349,6 +358,7 @@ class DeviceCodec:
         self.device = torch.device(device)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
+        self._index = self.device.index
         with torch.cuda.device(self.device):
             if not self.lib.svbgpu_device_ok():
                 raise SvbError("no usable gfx950 device")
@@ -481,7 +491,7 @@ class DeviceCodec:
         return kept[-1]
 
     def _norm_word(self, t, what):
-        if not (t.device == self.device and t.dtype == self.torch.float32 and t.numel() == 1):
+        if not (t.get_device() == self._index and t.dtype == self.torch.float32 and t.numel() == 1):
             raise ValueError(f"{what}: a one-element float32 tensor on {self.device}")
         if t.is_neg():
             raise ValueError(f"{what} is negated lazily: pass its resolve_neg()")
@@ -493,7 +503,7 @@ class DeviceCodec:
         codec share its workspaces: they, and replays of graphs that hold them, are ordered on one stream."""
         if norm_type not in NORMS:
             raise ValueError(f"norm_type {norm_type}: 1, 2 or inf")
-        grads = grads if isinstance(grads, GradSet) else GradSet(grads)
+        grads = grads if isinstance(grads, GradSet) else _OneCallSet(grads)
         grads._check(self.device)
         norm = self.torch.empty(1, dtype=self.torch.float32, device=self.device) if out is None else self._norm_word(out, "out")
         ws = self._grad_workspace(len(grads))
@@ -512,7 +522,7 @@ class DeviceCodec:
             raise ValueError(f"norm_type {norm_type}: 1, 2 or inf")
         if not max_norm >= 0:
             raise ValueError(f"max_norm {max_norm}")
-        grads = grads if isinstance(grads, GradSet) else GradSet(grads)
+        grads = grads if isinstance(grads, GradSet) else _OneCallSet(grads)
         grads._check(self.device)
         norm = self._norm_word(norm, "norm") if given else self.torch.empty(1, dtype=self.torch.float32, device=self.device)
         ws = self._grad_workspace(len(grads))
@@ -533,11 +543,11 @@ class DeviceCodec:
         if n > self.max_count:
             raise ValueError(f"{n} values, but the codec was made for {self.max_count}")
         residual_out = residual if residual_out is None else residual_out
-        device = self.device
+        device, index = self.device, self._index
         for t in (grad, residual, residual_out):
-            if t.device != device or not t.is_contiguous() or t.numel() != n:
+            if t.get_device() != index or not t.is_contiguous() or t.numel() != n:
                 raise ValueError(f"grad, residual and residual_out are contiguous tensors of {n} elements on {device}")
-            if t.is_neg():
+            if n == 1 and t.is_neg():  # longer ones are not contiguous
                 raise ValueError("a tensor is negated lazily: pass its resolve_neg()")
         if residual.dtype != torch.float32 or residual_out.dtype != torch.float32:
             raise ValueError("the residual is float32")
@@ -545,7 +555,7 @@ class DeviceCodec:
         written = [residual_out]
         if out is None:
             out = torch.empty(room, dtype=torch.uint8, device=device)
-        elif out.device != device or out.dtype != torch.uint8 or not out.is_contiguous() or out.numel() < room:
+        elif out.get_device() != index or out.dtype != torch.uint8 or not out.is_contiguous() or out.numel() < room:
             raise ValueError(f"out: a contiguous uint8 tensor of at least {room} bytes on {device}")
         else:
             written.append(out)

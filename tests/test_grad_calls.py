@@ -21,6 +21,7 @@ def dev(t):
 def codec():
     c = object.__new__(svb.DeviceCodec)
     c.torch, c.lib, c.device, c.max_count = torch, svb.load(), torch.device("cpu"), 1 << 20
+    c._index = -1  # what a host tensor says
     c.ws_bytes = c.lib.svbgpu_workspace_bytes(c.max_count)
     c.ws, c.res = torch.zeros(c.ws_bytes, dtype=torch.uint8), torch.zeros(8, dtype=torch.int64)
     c.calls = []
@@ -166,3 +167,15 @@ def test_lazily_negated_tensors_are_refused(codec):
     codec.grad_norm([dev(y)])
     codec.quantize_feedback_encode(y, 4.0, plain)
     assert len(codec.calls) == 2
+
+
+def test_versions_are_counted_once_a_buffer():
+    """A set that is kept holds one tensor for every version that its calls count on."""
+    bucket = torch.randn(100)
+    views = [dev(t) for t in bucket.split(10)]
+    others = [dev(torch.randn(10)) for _ in range(10)]
+    assert len(svb.GradSet(views).written) == 1 and len(svb.GradSet(others).written) == 10
+    assert len(svb.GradSet(others, out=views).written) == 1 and len(svb.GradSet(views, out=others).written) == 10
+    with torch.inference_mode():
+        made = [dev(t) for t in torch.randn(100).split(10)]
+    assert len(svb.GradSet(made).written) == 0
