@@ -278,15 +278,17 @@ typedef struct svbgpu_tensor {
 
 size_t svbgpu_grad_workspace_bytes(uint32_t ntensors);
 
-/* *d_norm = the norm of all elements of all tensors together.  Squares and sums are in 64 bits and the result is
- * rounded once: large and tiny elements neither overflow nor vanish, and the same tensors give the same bits every
- * time.  0 without elements; NaN if any element is NaN.  The tensors may overlap (an element counts each time). */
+/* *d_norm = the norm of all elements of all tensors together.  Squares and sums are in 64 bits and only the result is
+ * rounded to float32: large and tiny elements neither overflow nor vanish, and the norm is off by half a float32 step and
+ * the error of the 64-bit sum, n * 2^-53 of it at most.  The order of the sums follows from the tensors' sizes, types and
+ * order, so the same tensors in the same order give the same bits every time; in another order the last bit may differ.
+ * 0 without elements; NaN if any element is NaN.  The tensors may overlap (an element counts each time). */
 int svbgpu_grad_norm(int norm, const svbgpu_tensor *tensors, uint32_t ntensors, float *d_norm,
                      void *d_workspace, size_t workspace_bytes, void *stream);
 
 /* Clips by the global norm N: every element becomes x * c, c = 1 where N + 1e-6 <= max_norm, else
  * max_norm / (N + 1e-6) (64 bits, rounded once to float32; the product is rounded to float32 and then to the
- * tensor's type).  N not a number makes every element NaN; N infinite makes c zero.  outs == NULL: in place, and
+ * tensor's type).  N not a number makes every element NaN; N infinite makes c zero, unless max_norm is infinite too.  outs == NULL: in place, and
  * with c = 1 nothing is written; else tensor i goes to outs[i], of the same type and length, which may be the
  * tensor itself.  norm_given == 0: N is worked out as by svbgpu_grad_norm and left in *d_norm; norm_given != 0: N is
  * read from *d_norm (worked out before, or summed over ranks) and neither `norm` nor the workspace is used.

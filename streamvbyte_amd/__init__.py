@@ -263,9 +263,14 @@ class GradSet:
     """The tensors of one grad_norm / clip_grads call, looked over once and laid out as the C ABI takes them.
 
     `tensors`: float32, float16 and bfloat16 tensors of one device, mixed as they come, each dense in memory (any
-    order of dimensions).  `out`: tensors of the same types, shapes and strides that clip_grads writes instead.  A program whose
-    gradients keep their memory from step to step makes one GradSet and passes it to every call; it holds the
-    tensors, and raises if one of them has moved since.  Passing a plain list makes one on the spot."""
+    order of dimensions).  `out`: tensors of the same types, shapes and strides that clip_grads writes instead.
+
+    A set stands for memory: that which the tensors had when it was made, which it keeps alive.  It is for programs
+    whose gradients keep their memory from step to step (one bucket, or zero_grad(set_to_none=False)); they make one and
+    pass it to every call.  A tensor that is given other memory later (`x.data = ...`), or a gradient that is dropped
+    and made anew (zero_grad() does that), is not followed and cannot be noticed: the calls go on with the old memory.
+    There, pass a plain list, or make the set again.  What is noticed is a storage that has moved or given its memory
+    back: the call raises."""
 
     _kept = True  # made by the caller, for many calls
 
@@ -499,8 +504,10 @@ class DeviceCodec:
 
     def grad_norm(self, grads, norm_type=2.0, out=None):
         """Global norm of all elements of `grads` (a GradSet or a list of tensors) -> float32 tensor[1], asynchronously.
-        norm_type 2, 1 or inf.  Sums are in 64 bits, the result is rounded once; the same bits every time.  Calls of one
-        codec share its workspaces: they, and replays of graphs that hold them, are ordered on one stream."""
+        norm_type 2, 1 or inf.  Sums are in 64 bits, only the result is rounded to float32; one set gives the same bits
+        every time (tensors are summed in the order of their memory, so the same values elsewhere may differ in the last
+        bit).  Calls of one codec share its workspaces: they, and replays of graphs that hold them, are ordered on one
+        stream."""
         if norm_type not in NORMS:
             raise ValueError(f"norm_type {norm_type}: 1, 2 or inf")
         grads = grads if isinstance(grads, GradSet) else _OneCallSet(grads)
@@ -515,7 +522,8 @@ class DeviceCodec:
     def clip_grads(self, grads, max_norm, norm_type=2.0, norm=None):
         """Multiplies every element of `grads` (a GradSet or a list of tensors) by min(1, max_norm / (N + 1e-6)), N their
         global norm, in place or into the GradSet's `out` tensors; returns N, a float32 tensor[1].  `norm`: N worked out
-        before (over other ranks' shards too, say); it is then read instead, and returned, and norm_type is not looked at."""
+        before (over other ranks' shards too, say); it is then read instead, and returned, and norm_type is not looked at.
+        What is written counts as written in place: autograd refuses to go back through a graph that saved it."""
         given = norm is not None
         kind = 2 if given else NORMS.get(norm_type)
         if kind is None:

@@ -123,8 +123,8 @@ __device__ __forceinline__ GradChunk find_chunk(const GradTable<N>& t, u32 chunk
 
 // ---- norm -------------------------------------------------------------------------------------------------
 // N = (sum |x|^p)^(1/p) over every element of every tensor.  Squares and sums are in 64 bits: the square of a float32
-// is exact there and neither overflows nor vanishes, and the order of the sums cannot be seen after the one rounding
-// at the end.  The maximum is taken on the bits of |x|, where NaN stands above everything.
+// is exact there and neither overflows nor vanishes.  The order of the sums is that of the chunks, lanes and waves, the
+// same in every run; another order of the tensors may change the last bits of 64, and so, seldom, the last of 32.  The maximum is taken on the bits of |x|, where NaN stands above everything.
 template <int KIND>
 struct NormSum {
   double s0 = 0.0, s1 = 0.0;  // two chains of additions
@@ -509,8 +509,7 @@ constexpr u32 kFeedMaxWaves = 15;  // data waves of a workgroup, at most
 // is passed by a writer of the round that takes the same place.  Between a tile's ticket and its publication a workgroup
 // waits only for tiles with smaller tickets: the chain ends.
 //
-// Bound by memory, 12.8 B a value for float32 (0124): 2^26 values in 140 us = 6.2 TB/s; nothing but the elementwise part
-// takes 134.  What it took to get there from 187 us, the tile-at-a-time form of k_encode: assembling before the place is
+// Bound by memory, 12.8 B a value for float32 (0124): 2^26 values in 140 us = 6.2 TB/s.  What it took to get there from 187 us, the tile-at-a-time form of k_encode: assembling before the place is
 // known (165), half the instructions a value (feed_group, the one-byte quarters of assemble), one workgroup of 15 data
 // waves per CU instead of two (158; a look-back takes the longer the more tiles are in flight, about 20 ns each), the
 // deferred copy (144; 30 wave tiles a tile without it 151), 256 tile words a look-back instead of 128 (140: all that are

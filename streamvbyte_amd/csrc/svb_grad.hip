@@ -225,8 +225,10 @@ void launch_feedback(const void* grad, uint32_t count, uint8_t* d_out, const Fee
 //     12 * 2^20: 1x15 40.6, 2x12 37.3, deferred 35.6         2^24: 1x15 51.2, 2x12 48.7, deferred 45.0
 //     2^26: 1x15 163, 2x15 152, deferred 140
 // Two wave tiles a wave are for streams that are one round of the device's 256 CUs that way and more with one.
-// Non-temporal stores where what a call touches begins to fill the Infinity Cache, non-temporal loads where it is far
-// beyond it (deferred: 2^23 27.9 us, with such stores 25.3, with the loads too 27.4; 2^24 47.5, 45.0, 44.2).
+// Non-temporal stores from 7 * 2^19 values (47 MB read and written, 40 MB with 16-bit gradients), non-temporal loads from
+// 2^24 (215 and 180 MB): deferred, 2^23 27.9 us, with such stores 25.3, with the loads too 27.4; 2^24 47.5, 45.0, 44.2.
+// What reads the stream or the residual next has not been timed with either.  16-bit gradients and 1234 go by the same
+// counts, which were not measured for them.
 template <int V, int T>
 void launch_feedback(const void* grad, uint32_t count, uint8_t* d_out, const FeedArgs& fa, void* ws, unsigned tag2, uint64_t* d_written,
                      hipStream_t st) {
